@@ -39,13 +39,16 @@ enum wan_status {
   WAN_ERR_LAUNCH = 4       /* the HIP runtime rejected a launch */
 };
 
-/* A [batch, token, head, head_dim] bf16 device tensor. */
+/* A [batch, token, head, head_dim] device tensor (bf16, or of the call's dtype). */
 typedef struct wan_tensor {
   void* data;
   int64_t batch_stride;
   int64_t token_stride;
   int64_t head_stride;
 } wan_tensor;
+
+/* Element types, where an entry point takes one (`dtype`); all others are bf16. */
+enum wan_dtype { WAN_BF16 = 0, WAN_F16 = 1, WAN_F32 = 2 };
 
 /* Message of the calling thread's last failed call ("" if none). */
 const char* wan_attn_last_error(void);
@@ -204,6 +207,24 @@ int wan_rms_norm_qk(wan_tensor q, wan_tensor k, void* k_out, int batch, int seql
 int wan_rms_norm_qk_sumsq(wan_tensor k, void* k_out, int batch, int seqlen, int heads, int head_dim,
                           const void* gamma_k, float eps, const float* rope_cos, const float* rope_sin,
                           const float* sumsq, float* inv_rms_q, void* stream);
+
+/*
+ * RMSNorm of every head of q and k, and the rotation by position, in one pass over both.  No
+ * counterpart in the reference, whose norm spans all heads of a token (wan_rms_norm):
+ *   t = x * rsqrt(mean over the head's channels of x^2 + eps) * gamma
+ *   (t_a, t_b) -> (t_a cos - t_b sin, t_a sin + t_b cos)  in fp32, one rounding at the end
+ * q [batch, seqlen, heads_q, head_dim] and k [.., heads_k, ..] of type dtype, head_dim a multiple of
+ * 8 up to 256; q_out and k_out contiguous, not overlapping the inputs; gamma [head_dim] of the same
+ * type.  rope_cos / rope_sin: fp32 [table_rows, rope_pairs], NULL: no rotation.  The pairs are channels
+ * (2j, 2j+1) (interleaved != 0, rope_pairs a multiple of 4) or (j, j + rope_pairs) (a multiple of
+ * 8); channels from 2 * rope_pairs on are not turned.  A token's table row is positions[b, l] (device
+ * int32, NULL: l); where the tables have no such row, the token's q_out and k_out are NaN.
+ */
+int wan_head_norm_rope(wan_tensor q, wan_tensor k, void* q_out, void* k_out, int batch, int seqlen,
+                       int heads_q, int heads_k, int head_dim, int dtype, const void* gamma_q,
+                       const void* gamma_k, float eps, const float* rope_cos, const float* rope_sin,
+                       int table_rows, int rope_pairs, const int32_t* positions, int interleaved,
+                       void* stream);
 
 /*
  * Attention whose query is normalised inside the kernel as it is loaded:

@@ -512,6 +512,71 @@ int wan_rope(wan_tensor x, void* out, int batch, int seqlen, int heads, int head
   return launch_rope(a, static_cast<hipStream_t>(stream));
 }
 
+int wan_head_norm_rope(wan_tensor q, wan_tensor k, void* q_out, void* k_out, int batch, int seqlen, int heads_q,
+                       int heads_k, int head_dim, int dtype, const void* gamma_q, const void* gamma_k, float eps,
+                       const float* rope_cos, const float* rope_sin, int table_rows, int rope_pairs,
+                       const int32_t* positions, int interleaved, void* stream) {
+  const char* fn = "wan_head_norm_rope";
+  int rc;
+  if (batch < 0 || seqlen < 0 || heads_q < 0 || heads_k < 0)
+    return set_error(WAN_ERR_INVALID, "%s: negative size (batch=%d seqlen=%d heads=%d, %d)", fn, batch, seqlen,
+                     heads_q, heads_k);
+  if (head_dim <= 0 || head_dim % 8 != 0 || head_dim > 256)
+    return set_error(WAN_ERR_UNSUPPORTED, "%s: head_dim=%d must be a multiple of 8 and <= 256", fn, head_dim);
+  if (dtype != WAN_BF16 && dtype != WAN_F16 && dtype != WAN_F32)
+    return set_error(WAN_ERR_UNSUPPORTED, "%s: dtype=%d is none of WAN_BF16, WAN_F16, WAN_F32", fn, dtype);
+  if (heads_q > (1 << 20) || heads_k > (1 << 20) || (int64_t)batch * seqlen > 0x7fffffff)
+    return set_error(WAN_ERR_UNSUPPORTED, "%s: %lld tokens or %d + %d heads is too many", fn,
+                     (long long)batch * seqlen, heads_q, heads_k);
+  if ((rc = check_tensor(fn, "q", q, batch, seqlen, heads_q))) return rc;
+  if ((rc = check_tensor(fn, "k", k, batch, seqlen, heads_k))) return rc;
+  if ((int64_t)batch * seqlen * ((int64_t)heads_q + heads_k) == 0) return WAN_OK;
+  if ((heads_q > 0 && !q_out) || (heads_k > 0 && !k_out) || !aligned16(q_out) || !aligned16(k_out))
+    return set_error(WAN_ERR_INVALID, "%s: q_out and k_out must be 16-byte aligned pointers", fn);
+  if (!gamma_q || !gamma_k || !aligned16(gamma_q) || !aligned16(gamma_k))
+    return set_error(WAN_ERR_INVALID, "%s: gamma_q and gamma_k must be 16-byte aligned pointers", fn);
+  if (!(eps >= 0.f)) return set_error(WAN_ERR_INVALID, "%s: eps must be >= 0", fn);
+  if ((rope_cos == nullptr) != (rope_sin == nullptr))
+    return set_error(WAN_ERR_INVALID, "%s: rope_cos and rope_sin must both be given or both NULL", fn);
+  if (positions && !rope_cos) return set_error(WAN_ERR_INVALID, "%s: positions given without tables", fn);
+  if (rope_cos) {
+    if (!aligned16(rope_cos) || !aligned16(rope_sin))
+      return set_error(WAN_ERR_INVALID, "%s: rope tables must be 16-byte aligned", fn);
+    const int unit = interleaved ? 4 : 8;
+    if (rope_pairs <= 0 || rope_pairs % unit != 0 || 2 * (int64_t)rope_pairs > head_dim)
+      return set_error(WAN_ERR_UNSUPPORTED, "%s: rope_pairs=%d must be a multiple of %d, at most head_dim / 2", fn,
+                       rope_pairs, unit);
+    if (table_rows <= 0 || (!positions && table_rows < seqlen))
+      return set_error(WAN_ERR_INVALID, "%s: the tables have %d rows for %d tokens", fn, table_rows, seqlen);
+  }
+  HeadNormArgs a{};
+  a.q = q.data;
+  a.k = k.data;
+  a.q_sb = q.batch_stride;
+  a.q_st = q.token_stride;
+  a.q_sh = q.head_stride;
+  a.k_sb = k.batch_stride;
+  a.k_st = k.token_stride;
+  a.k_sh = k.head_stride;
+  a.q_out = q_out;
+  a.k_out = k_out;
+  a.B = batch;
+  a.L = seqlen;
+  a.Hq = heads_q;
+  a.Hk = heads_k;
+  a.D = head_dim;
+  a.gamma_q = gamma_q;
+  a.gamma_k = gamma_k;
+  a.eps = eps;
+  a.cos = rope_cos;
+  a.sin = rope_sin;
+  a.rows = table_rows;
+  a.P = rope_pairs;
+  a.positions = positions;
+  a.interleaved = interleaved != 0;
+  return launch_head_norm(a, dtype, static_cast<hipStream_t>(stream));
+}
+
 size_t wan_qkv_proj_workspace(int M, int N, int K) {
   return M > 0 && N > 0 && K > 0 && N % 256 == 0 && K % 64 == 0 ? gemm_split_bytes(M, N, K) : 0;
 }

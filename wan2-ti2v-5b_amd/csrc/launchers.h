@@ -57,6 +57,31 @@ struct RopeArgs {
 };
 int launch_rope(const RopeArgs& a, hipStream_t s);
 
+// Element types at the C ABI (wan_dtype).
+enum Dtype { kBF16 = 0, kF16 = 1, kF32 = 2 };
+
+// RMSNorm of every head of q and k and the rotation by position.
+struct HeadNormArgs {
+  const void* q;        // [B, L, Hq, D] by strides
+  const void* k;        // [B, L, Hk, D]
+  int64_t q_sb, q_st, q_sh, k_sb, k_st, k_sh;
+  void* q_out;          // contiguous
+  void* k_out;
+  int B, L, Hq, Hk, D;  // D a multiple of 8, up to 256
+  const void* gamma_q;  // [D]
+  const void* gamma_k;
+  float eps;
+  const float* cos;     // [rows, P] (null: no rotation)
+  const float* sin;
+  int rows, P;
+  const int32_t* positions;  // [B, L] table rows (null: the token's place l)
+  bool interleaved;     // pairs (2j, 2j + 1), else (j, j + P)
+  // set by the launcher (HeadNormPlan)
+  unsigned grid_x;
+  int waves_per_token, slot_shift, token_shift;
+};
+int launch_head_norm(const HeadNormArgs& a, int dtype, hipStream_t s);
+
 // One adaLN stage of a block: residual update, LayerNorm, per-frame modulation.
 struct AdaLNArgs {
   const bf16* x;        // [B, L, C] residual stream

@@ -73,6 +73,45 @@ inline RowGrid row_grid(int64_t blocks, int threads) {
 }
 
 // ---------------------------------------------------------------------------
+// the norms of q and k heads (head_norm.hip)
+// ---------------------------------------------------------------------------
+
+// A wave holds 64 / lanes heads at once.  2^slot_shift of them are one token's, of 2^token_shift tokens;
+// a token's heads are `waves_per_token` waves with `chunks` such steps each.
+struct HeadNormPlan {
+  int waves_per_token, slot_shift, token_shift;
+  int64_t waves;
+};
+inline HeadNormPlan head_norm_plan(int64_t tokens, int heads, int lanes, int chunks) {
+  HeadNormPlan p{};
+  int slots = 0;
+  while ((64 / lanes) >> (slots + 1)) ++slots;
+  while (p.slot_shift < slots && (1 << p.slot_shift) < heads) ++p.slot_shift;
+  p.token_shift = slots - p.slot_shift;
+  const int per_wave = chunks << p.slot_shift;
+  p.waves_per_token = (heads + per_wave - 1) / per_wave;
+  const int64_t groups = (tokens + (1 << p.token_shift) - 1) >> p.token_shift;
+  p.waves = groups * p.waves_per_token;
+  return p;
+}
+// Heads a lane works on: one where the launch then still has few waves, else as leaves the fewest lanes
+// without a head, the larger of equals.
+constexpr int64_t kFewWaves = 4096;
+inline int head_norm_chunks(int64_t tokens, int heads, int lanes) {
+  if (head_norm_plan(tokens, heads, lanes, 1).waves <= kFewWaves) return 1;
+  int best = 1;
+  int64_t least = -1;
+  for (int n = 4; n >= 1; --n) {
+    const int64_t lanes_used = head_norm_plan(tokens, heads, lanes, n).waves * n;
+    if (least < 0 || lanes_used < least) {
+      least = lanes_used;
+      best = n;
+    }
+  }
+  return best;
+}
+
+// ---------------------------------------------------------------------------
 // the projection GEMM (gemm.hip)
 // ---------------------------------------------------------------------------
 

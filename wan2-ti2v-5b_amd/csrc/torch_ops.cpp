@@ -317,6 +317,57 @@ void rms_inv(const OperatorHandle& op, DispatchKeySet ks, Stack* stack) {
   c.give(std::move(inv));
 }
 
+// [B, L, heads, D], the channels contiguous
+bool heads4(const Tensor& t, at::ScalarType type, int64_t D, c10::Device dev) {
+  return plain(t, type, dev) && t.dim() == 4 && t.size(3) == D && t.numel() > 0 && small_int(t.size(0)) &&
+         small_int(t.size(1)) && small_int(t.size(2)) && t.stride(3) == 1 && t.stride(0) % 8 == 0 &&
+         t.stride(1) % 8 == 0 && t.stride(2) % 8 == 0 && aligned(t);
+}
+
+// enum wan_dtype, or -1
+int dtype_of(const Tensor& t) {
+  switch (t.scalar_type()) {
+    case at::kBFloat16: return WAN_BF16;
+    case at::kHalf: return WAN_F16;
+    case at::kFloat: return WAN_F32;
+    default: return -1;
+  }
+}
+
+// head_norm_rope(q, k, gamma_q, gamma_k, eps, cos?, sin?, positions?, interleaved)
+void head_norm_rope(const OperatorHandle& op, DispatchKeySet ks, Stack* stack) {
+  Call c(op, stack);
+  const Tensor &q = c.tensor(0), &k = c.tensor(1);
+  const auto dev = q.device();
+  const int type = dtype_of(q);
+  bool ok = dev.is_cuda() && type >= 0 && q.dim() == 4 && k.dim() == 4 && heads4(q, q.scalar_type(), q.size(3), dev) &&
+            heads4(k, q.scalar_type(), q.size(3), dev) && q.size(0) == k.size(0) && q.size(1) == k.size(1) &&
+            q.size(3) % 8 == 0 && q.size(3) <= 256 && vec(c.tensor(2), q.size(3), q.scalar_type(), dev) &&
+            vec(c.tensor(3), q.size(3), q.scalar_type(), dev) && c.has(5) == c.has(6) && (c.has(5) || !c.has(7));
+  int rows = 0, pairs = 0;
+  if (ok && c.has(5)) {
+    const Tensor &cos = c.tensor(5), &sin = c.tensor(6);
+    ok = cos.dim() == 2 && cos.sizes() == sin.sizes() && vec(cos, cos.numel(), at::kFloat, dev) &&
+         vec(sin, cos.numel(), at::kFloat, dev) && small_int(cos.size(0)) && small_int(cos.size(1));
+    if (ok) {
+      rows = (int)cos.size(0);
+      pairs = (int)cos.size(1);
+    }
+    if (ok && c.has(7))
+      ok = c.tensor(7).dim() == 2 && c.tensor(7).size(0) == q.size(0) && c.tensor(7).size(1) == q.size(1) &&
+           vec(c.tensor(7), q.size(0) * q.size(1), at::kInt, dev);
+  }
+  if (!ok) return to_python(op, ks, stack);
+  const Site s(q);
+  Tensor q_out = s.rows(q), k_out = s.rows(k);
+  check("wan_head_norm_rope",
+        wan_head_norm_rope(t4(q), t4(k), q_out.data_ptr(), k_out.data_ptr(), (int)q.size(0), (int)q.size(1),
+                           (int)q.size(2), (int)k.size(2), (int)q.size(3), type, c.ptr(2), c.ptr(3), c.real(4),
+                           static_cast<const float*>(c.ptr(5)), static_cast<const float*>(c.ptr(6)), rows, pairs,
+                           static_cast<const int32_t*>(c.ptr(7)), c[8].toBool(), s.stream()));
+  c.give(std::move(q_out), std::move(k_out));
+}
+
 // adaln(x, y?, e?, frames, gate_idx, shift_idx, scale_idx, ln_weight?, ln_bias?, eps, norm, e_mod?)
 void adaln(const OperatorHandle& op, DispatchKeySet ks, Stack* stack) {
   Call c(op, stack);
@@ -396,7 +447,7 @@ void linear(const OperatorHandle& op, DispatchKeySet ks, Stack* stack) {
   X("flash_self_attn", flash_self_attn) X("cross_attn", cross_attn) X("self_attn_fused", self_attn_fused) \
   X("self_attn_fused_sumsq", self_attn_fused_sumsq) X("cross_attn_fused", cross_attn_fused)         \
   X("flash_attn_qnorm", flash_attn_qnorm) X("rope", rope_op) X("rms_norm", rms_norm) X("rms_inv", rms_inv) \
-  X("adaln", adaln) X("qkv_proj_sumsq", qkv_proj_sumsq) X("linear", linear)
+  X("head_norm_rope", head_norm_rope) X("adaln", adaln) X("qkv_proj_sumsq", qkv_proj_sumsq) X("linear", linear)
 
 TORCH_LIBRARY_IMPL(wan_hip, CUDA, m) {
 #define WAN_IMPL(name, fn) m.impl(name, torch::CppFunction::makeFromBoxedFunction<&defined<&fn>>());

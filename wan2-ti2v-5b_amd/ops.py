@@ -302,6 +302,82 @@ def _(q, k, v, inv_rms_q, gamma_q, cos, sin, seqlen_k, softmax_scale):
     return q.new_empty(q.shape)
 
 
+# ─── norms of q and k heads with the rotation ──────────────────────────────────
+
+_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}      # enum wan_dtype
+
+
+def _check_heads(name: str, x: torch.Tensor, dims, dtypes) -> None:
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"{name}: expected a tensor, got {type(x).__name__}")
+    if x.dim() != 4:
+        raise ValueError(f"{name}: expected [B, L, heads, head_dim], got shape {tuple(x.shape)}")
+    if x.device.type != "cuda":
+        raise ValueError(f"{name}: expected a CUDA (HIP) tensor, got device {x.device}")
+    if x.dtype not in dtypes:
+        raise ValueError(f"{name}: expected one of {[str(t) for t in dtypes]}, got {x.dtype}")
+    if x.shape[-1] not in dims:
+        raise ValueError(f"{name}: head_dim {x.shape[-1]} is not implemented ({dims})")
+    if x.numel() == 0:
+        return
+    if x.stride(-1) != 1:
+        raise ValueError(f"{name}: the head_dim axis must be contiguous (stride {x.stride(-1)})")
+    if any(s % 8 for s in x.stride()[:3]) or x.data_ptr() % 16:
+        raise ValueError(f"{name}: strides {x.stride()} must be multiples of 8 elements "
+                         "and the data 16-byte aligned")
+
+
+@torch.library.custom_op("wan_hip::head_norm_rope", mutates_args=())
+def head_norm_rope(q: torch.Tensor, k: torch.Tensor, gamma_q: torch.Tensor, gamma_k: torch.Tensor, eps: float,
+                   cos: Optional[torch.Tensor] = None, sin: Optional[torch.Tensor] = None,
+                   positions: Optional[torch.Tensor] = None,
+                   interleaved: bool = True) -> Tuple[torch.Tensor, torch.Tensor]:
+    """RMSNorm of every head of q [B, L, Hq, D] and k [B, L, Hk, D] (bf16, fp16 or fp32; D a multiple
+    of 8 up to 256; gamma [D]) and the rotation of its first 2 P channels by cos / sin fp32 [n, P], in
+    one pass and with one rounding.  Pairs are channels (2j, 2j+1), or (j, j + P) with interleaved
+    False.  A token's table row is positions[b, l] (int32 [B, L]), by default l; a token whose row the
+    tables do not hold becomes NaN."""
+    fn = "head_norm_rope"
+    dims = range(8, 257, 8)
+    for name, t in (("q", q), ("k", k)):
+        _check_heads(f"{fn}: {name}", t, dims, tuple(_DTYPES))
+    if q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3] or q.dtype != k.dtype or q.device != k.device:
+        raise ValueError(f"{fn}: q {q.dtype} {tuple(q.shape)} on {q.device} and k {k.dtype} {tuple(k.shape)} on "
+                         f"{k.device} disagree")
+    B, L, Hq, D = q.shape
+    for name, t in (("gamma_q", gamma_q), ("gamma_k", gamma_k)):
+        _check_vec(fn, name, t, D, q.dtype, q.device)
+    if (cos is None) != (sin is None):
+        raise ValueError(f"{fn}: give both cos and sin, or neither")
+    if cos is None and positions is not None:
+        raise ValueError(f"{fn}: positions without cos and sin")
+    rows = pairs = 0
+    if cos is not None:
+        if cos.dim() != 2 or cos.shape != sin.shape:
+            raise ValueError(f"{fn}: cos {tuple(cos.shape)} and sin {tuple(sin.shape)} must be [rows, pairs] alike")
+        rows, pairs = cos.shape
+        for name, t in (("cos", cos), ("sin", sin)):
+            _check_vec(fn, name, t, rows * pairs, torch.float32, q.device)
+        if positions is not None:
+            if positions.shape != (B, L):
+                raise ValueError(f"{fn}: positions must be [{B}, {L}], got {tuple(positions.shape)}")
+            _check_vec(fn, "positions", positions, B * L, torch.int32, q.device)
+    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    with torch.cuda.device(q.device):
+        N.check("wan_head_norm_rope", N.lib().wan_head_norm_rope(
+            N.tensor4(q), N.tensor4(k), q_out.data_ptr(), k_out.data_ptr(), B, L, Hq, k.shape[2], D, _DTYPES[q.dtype],
+            gamma_q.data_ptr(), gamma_k.data_ptr(), float(eps), None if cos is None else cos.data_ptr(),
+            None if sin is None else sin.data_ptr(), rows, pairs, None if positions is None else positions.data_ptr(),
+            int(interleaved), _stream(q.device)))
+    return q_out, k_out
+
+
+@head_norm_rope.register_fake
+def _(q, k, gamma_q, gamma_k, eps, cos=None, sin=None, positions=None, interleaved=True):
+    return q.new_empty(q.shape), k.new_empty(k.shape)
+
+
 # ─── adaLN: the pointwise stages of a WanAttentionBlock ─────────────────────
 
 def _check_rows(fn: str, name: str, t: torch.Tensor, shape, device) -> None:
