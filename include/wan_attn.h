@@ -113,6 +113,40 @@ int wan_flash_attn_qnorm_ws(wan_tensor q, wan_tensor k, wan_tensor v, wan_tensor
                             void* workspace, size_t workspace_bytes, void* stream);
 
 /*
+ * Attention under masks, with as many or fewer k/v heads than query heads.  No counterpart in the
+ * reference.  q, out [batch, seqlen_q, heads_q, head_dim], k, v [batch, seqlen_k, heads_k, head_dim] of
+ * type dtype (WAN_BF16 or WAN_F16), head_dim 64 or 128, heads_q a multiple of heads_k: query head h reads
+ * k/v head h / (heads_q / heads_k).  With the parts of `mask` that are not NULL / 0 (mask NULL: none):
+ *   p_i  = q_start[b] + i                  the position of query row i among the keys
+ *   s_ij = softmax_scale q_i . k_j;  s = softcap tanh(s / softcap);  s += bias[h, clamp(j - p_i, -R, R) + R]
+ *   row i sees key j if j < seqlen_k[b], and j and p_i are of one document, and (causal) j <= p_i or j is
+ *   in the first prefix_lens of them
+ *   out_i  = softmax over the keys seen of s_i, times v;  zeros where no key is seen, or all of them at -inf
+ * v rows of keys that a row does not see do not reach it, whatever they hold.  The arrays are on the device
+ * and int32: values outside their ranges are clamped, doc_starts that do not ascend give other documents,
+ * never a read out of range.  `workspace` is optional scratch of wan_masked_attn_workspace() bytes, 256-byte
+ * aligned (0: not needed): with it calls of few rows split their keys over the compute units, with
+ * fewer bytes less far.
+ */
+typedef struct wan_attn_mask {
+  int causal;
+  float softcap;               /* 0: none; finite, >= 0 */
+  const float* bias;           /* [heads_q, 2 bias_reach + 1] fp32; finite or -inf (hides the key) */
+  int bias_reach;              /* R: distances beyond it have the bias of R */
+  const int32_t* doc_starts;   /* [batch, docs] first positions, ascending; a document ends where the next
+                                  begins; positions before the first are of no document */
+  int docs;
+  const int32_t* prefix_lens;  /* [batch], with doc_starts [batch, docs]; causal only */
+  const int32_t* seqlen_k;     /* [batch]; NULL: seqlen_k for all */
+  const int32_t* q_start;      /* [batch], within +- 2^30; NULL: seqlen_k - seqlen_q (the argument's), so that
+                                  the last row is at the last key */
+} wan_attn_mask;
+size_t wan_masked_attn_workspace(int batch, int heads_q, int heads_k, int seqlen_q, int seqlen_k, int head_dim);
+int wan_masked_attn(wan_tensor q, wan_tensor k, wan_tensor v, wan_tensor out, int batch, int heads_q,
+                    int heads_k, int seqlen_q, int seqlen_k, int head_dim, int dtype, float softmax_scale,
+                    const wan_attn_mask* mask, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Fused self-attention span of _FastBlock.forward, models/fast_dit.py:281-292:
  *   q,k = _tp_rms_qk(q, k) (RMS over all heads*128 channels of a token, eps,
  *         bf16 gamma [heads*128]); q,k = _rope(q), _rope(k); out = attention(q, k, v).

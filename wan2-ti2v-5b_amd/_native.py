@@ -29,6 +29,21 @@ class WanTensor(ctypes.Structure):
     ]
 
 
+class WanAttnMask(ctypes.Structure):
+    """struct wan_attn_mask: the masks and score changes of wan_masked_attn (device addresses, 0: none)."""
+    _fields_ = [
+        ("causal", ctypes.c_int),
+        ("softcap", ctypes.c_float),
+        ("bias", ctypes.c_void_p),
+        ("bias_reach", ctypes.c_int),
+        ("doc_starts", ctypes.c_void_p),
+        ("docs", ctypes.c_int),
+        ("prefix_lens", ctypes.c_void_p),
+        ("seqlen_k", ctypes.c_void_p),
+        ("q_start", ctypes.c_void_p),
+    ]
+
+
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _F = ctypes.c_float
@@ -55,6 +70,8 @@ SIGNATURES = {
     "wan_rope": (_I, [_T, _P, _I, _I, _I, _I, _P, _P, _P]),
     "wan_rms_norm": (_I, [_T, _P, _I, _I, _I, _I, _P, _F, _P, _P, _P, _P]),
     "wan_rms_norm_qk": (_I, [_T, _T, _P, _I, _I, _I, _I, _P, _F, _P, _P, _P, _P]),
+    "wan_masked_attn_workspace": (_SZ, [_I] * 6),
+    "wan_masked_attn": (_I, [_T, _T, _T, _T, _I, _I, _I, _I, _I, _I, _I, _F, ctypes.POINTER(WanAttnMask), _P, _SZ, _P]),
     "wan_head_norm_rope": (_I, [_T, _T, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P, _F, _P, _P, _I, _I, _P, _I, _P]),
     "wan_flash_attn_qnorm": (_I, [_T, _T, _T, _T, _I, _I, _I, _I, _I, _P, _P, _P, _P, _F, _P, _P]),
     "wan_adaln": (_I, [_P, _P, _P, _P, _I, _I, _I, _P, _I, _I, _I, _I, _P, _P, _F, _P]),

@@ -512,6 +512,78 @@ int wan_rope(wan_tensor x, void* out, int batch, int seqlen, int heads, int head
   return launch_rope(a, static_cast<hipStream_t>(stream));
 }
 
+size_t wan_masked_attn_workspace(int batch, int heads_q, int heads_k, int seqlen_q, int seqlen_k, int head_dim) {
+  if (heads_k <= 0 || heads_q % heads_k != 0 || (head_dim != 64 && head_dim != 128)) return 0;
+  return masked_split_bytes(batch, heads_q, heads_k, seqlen_q, seqlen_k, head_dim);
+}
+
+int wan_masked_attn(wan_tensor q, wan_tensor k, wan_tensor v, wan_tensor out, int batch, int heads_q, int heads_k,
+                    int seqlen_q, int seqlen_k, int head_dim, int dtype, float softmax_scale,
+                    const wan_attn_mask* mask, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* fn = "wan_masked_attn";
+  const wan_attn_mask none{};
+  const wan_attn_mask& m = mask != nullptr ? *mask : none;
+  int rc;
+  if ((rc = check_scale(fn, softmax_scale))) return rc;
+  if (batch < 0 || heads_q < 0 || heads_k < 0 || seqlen_q < 0 || seqlen_k < 0)
+    return set_error(WAN_ERR_INVALID, "%s: negative size (batch=%d heads=%d, %d Lq=%d Lk=%d)", fn, batch, heads_q,
+                     heads_k, seqlen_q, seqlen_k);
+  if (head_dim != 64 && head_dim != 128)
+    return set_error(WAN_ERR_UNSUPPORTED, "%s: head_dim=%d, 64 and 128 are implemented", fn, head_dim);
+  if (dtype != WAN_BF16 && dtype != WAN_F16)
+    return set_error(WAN_ERR_UNSUPPORTED, "%s: dtype=%d, WAN_BF16 and WAN_F16 are implemented", fn, dtype);
+  if (batch == 0 || heads_q == 0 || seqlen_q == 0) return WAN_OK;
+  if (heads_k == 0 || heads_q % heads_k != 0)
+    return set_error(WAN_ERR_INVALID, "%s: %d query heads are no multiple of %d k/v heads", fn, heads_q, heads_k);
+  if (seqlen_k > (1 << 30) || (int64_t)seqlen_q * (heads_q / heads_k) > (1 << 30))
+    return set_error(WAN_ERR_UNSUPPORTED, "%s: %d keys or %d rows of %d heads exceed 2^30", fn, seqlen_k, seqlen_q,
+                     heads_q / heads_k);
+  if ((rc = check_tensor(fn, "q", q, batch, seqlen_q, heads_q))) return rc;
+  if ((rc = check_tensor(fn, "k", k, batch, seqlen_k, heads_k))) return rc;
+  if ((rc = check_tensor(fn, "v", v, batch, seqlen_k, heads_k))) return rc;
+  if ((rc = check_tensor(fn, "out", out, batch, seqlen_q, heads_q))) return rc;
+  if (!(m.softcap >= 0.f) || !(m.softcap < INFINITY))
+    return set_error(WAN_ERR_INVALID, "%s: softcap=%g, must be finite and >= 0", fn, (double)m.softcap);
+  if (m.bias && (m.bias_reach < 0 || m.bias_reach > (1 << 29)))
+    return set_error(WAN_ERR_INVALID, "%s: bias_reach=%d must be in [0, 2^29]", fn, m.bias_reach);
+  if (m.doc_starts && m.docs <= 0) return set_error(WAN_ERR_INVALID, "%s: docs=%d, must be > 0", fn, m.docs);
+  if (m.prefix_lens && !m.causal)
+    return set_error(WAN_ERR_INVALID, "%s: prefix_lens without causal", fn);
+  const void* arrays[] = {m.bias, m.doc_starts, m.prefix_lens, m.seqlen_k, m.q_start};
+  for (const void* p : arrays)
+    if (reinterpret_cast<uintptr_t>(p) % 4)
+      return set_error(WAN_ERR_INVALID, "%s: the mask's arrays must be 4-byte aligned", fn);
+  if (workspace != nullptr && reinterpret_cast<uintptr_t>(workspace) % kAlign)
+    return set_error(WAN_ERR_INVALID, "%s: workspace must be 256-byte aligned", fn);
+  auto any4 = [](const wan_tensor& t) { return AnyTensor4{t.data, t.batch_stride, t.token_stride, t.head_stride}; };
+  MaskedArgs a{};
+  a.q = any4(q);
+  a.k = any4(k);
+  a.v = any4(v);
+  a.o = out.data;
+  a.o_sb = out.batch_stride;
+  a.o_st = out.token_stride;
+  a.o_sh = out.head_stride;
+  a.B = batch;
+  a.Hq = heads_q;
+  a.Hk = heads_k;
+  a.Lq = seqlen_q;
+  a.Lk = seqlen_k;
+  a.scale = softmax_scale;
+  a.cap = m.softcap;
+  a.causal = m.causal != 0;
+  a.bias = m.bias;
+  a.reach = m.bias_reach;
+  a.doc_starts = m.doc_starts;
+  a.docs = m.docs;
+  a.prefix_lens = m.prefix_lens;
+  a.seqlen_k = m.seqlen_k;
+  a.q_start = m.q_start;
+  a.part = static_cast<float*>(workspace);
+  a.part_bytes = workspace_bytes;
+  return launch_masked_attn(a, head_dim, dtype, static_cast<hipStream_t>(stream));
+}
+
 int wan_head_norm_rope(wan_tensor q, wan_tensor k, void* q_out, void* k_out, int batch, int seqlen, int heads_q,
                        int heads_k, int head_dim, int dtype, const void* gamma_q, const void* gamma_k, float eps,
                        const float* rope_cos, const float* rope_sin, int table_rows, int rope_pairs,

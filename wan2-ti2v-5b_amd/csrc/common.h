@@ -81,6 +81,33 @@ struct FlashArgs {
 int launch_flash_fwd(const FlashArgs& a, hipStream_t s);
 // Scratch bytes that a launch of this size makes use of (0: it does not split).
 size_t flash_split_bytes(int B, int H, int Lq, int Lk);
+
+// Attention under masks (masked_attn.h).
+struct AnyTensor4 {
+  const void* ptr;
+  int64_t sb, st, sh;
+};
+struct MaskedArgs {
+  AnyTensor4 q, k, v;
+  void* o;
+  int64_t o_sb, o_st, o_sh;
+  int B, Hq, Hk, Lq, Lk;     // Hq a multiple of Hk
+  float scale, cap;          // cap 0: none
+  bool causal;
+  const float* bias;         // [Hq, 2 reach + 1] by distance (null: none)
+  int reach;
+  const int32_t* doc_starts; // [B, docs] first keys of the documents, ascending (null: one document)
+  int docs;
+  const int32_t* prefix_lens;// [B], with documents [B, docs] (null: none; causal only)
+  const int32_t* seqlen_k;   // [B] (null: Lk)
+  const int32_t* q_start;    // [B] position of query row 0 (null: Lk - Lq)
+  float* part;               // scratch of the key split (null: none)
+  size_t part_bytes;
+  // set by the launcher (MaskedPlan)
+  int pack, splits, part_rows, part_floats;
+};
+int launch_masked_attn(MaskedArgs a, int D, int dtype, hipStream_t s);
+size_t masked_split_bytes(int B, int Hq, int Hk, int Lq, int Lk, int D);
 // CU count of the current device (cached per device after the first query).
 int device_cu_count();
 

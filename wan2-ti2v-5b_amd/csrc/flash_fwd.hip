@@ -1108,6 +1108,8 @@ int launch_qp(const FlashArgs& a, hipStream_t s) {
   return launch_nw<kWaves, QP>(a, s);
 }
 
+#include "masked_attn.h"
+
 }  // namespace
 
 // CU count of the current device, queried once per device (wan_attn_init() does that
@@ -1137,6 +1139,25 @@ int launch_flash_fwd(const FlashArgs& a, hipStream_t s) {
     case kQNormRope: return launch_qp<kQNormRope>(a, s);
     default: return set_error(1, "flash_fwd: unknown q preparation %d", a.qprep);
   }
+}
+
+size_t masked_split_bytes(int B, int Hq, int Hk, int Lq, int Lk, int D) {
+  if (B <= 0 || Hq <= 0 || Hk <= 0 || Lq <= 0 || Lk <= 0) return 0;
+  return masked_plan(B, Hq, Hk, Lq, Lk, D, device_cu_count(), SIZE_MAX).bytes;
+}
+
+int launch_masked_attn(MaskedArgs a, int D, int dtype, hipStream_t s) {
+  if (a.B == 0 || a.Hq == 0 || a.Lq == 0) return 0;
+  const MaskedPlan p = masked_plan(a.B, a.Hq, a.Hk, a.Lq, a.Lk, D, device_cu_count(),
+                                   a.part != nullptr ? a.part_bytes : 0);
+  if (p.blocks * p.splits > 0x7fffffff || p.out_rows > 0x7fffffff)
+    return set_error(2, "masked_attn: %lld workgroups is too many", (long long)p.blocks * p.splits);
+  a.pack = p.pack;
+  a.splits = p.splits;
+  a.part_rows = p.part_rows;
+  a.part_floats = p.part_floats;
+  if (dtype == 1) return D == 64 ? launch_masked_map<_Float16, 64>(a, p, s) : launch_masked_map<_Float16, 128>(a, p, s);
+  return D == 64 ? launch_masked_map<bf16, 64>(a, p, s) : launch_masked_map<bf16, 128>(a, p, s);
 }
 
 }  // namespace wan

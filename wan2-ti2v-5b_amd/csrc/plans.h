@@ -54,6 +54,47 @@ inline SplitPlan split_plan(int B, int H, int Lq, int keys, int cus, size_t scra
 }
 
 // ---------------------------------------------------------------------------
+// the attention under masks (masked_attn.h)
+// ---------------------------------------------------------------------------
+
+// Sizes up to this (keys, query rows of a sample over their heads) and positions of the first query row
+// within +- this keep every position and distance in 32 bits.
+constexpr int kMaxPosition = (1 << 30) - 1;
+// Caps above this take the form of the tanh that is exact for small arguments too.
+constexpr float kExactCap = 256.f;
+// Query heads that are rows beside each other, at most (a tile has 32 rows).
+constexpr int kMaxPack = 32;
+
+// How a call is run: `pack` query heads of one k/v head are rows of a block, `blocks` blocks of block_rows
+// rows, each as `splits` workgroups over a part of its keys.  A part's result: part_rows rows of D fp32,
+// their maxima and their sums.
+struct MaskedPlan {
+  int pack, block_rows, splits, part_rows, part_floats;
+  int64_t blocks, out_rows;
+  size_t bytes;
+};
+inline MaskedPlan masked_plan(int B, int Hq, int Hk, int Lq, int Lk, int D, int cus, size_t scratch) {
+  MaskedPlan p{};
+  const int group = Hq / Hk;
+  p.pack = group < kMaxPack ? group : kMaxPack;
+  while (group % p.pack != 0) --p.pack;
+  p.block_rows = 32;
+  const int64_t rows = (int64_t)Lq * p.pack;
+  p.blocks = (rows + p.block_rows - 1) / p.block_rows * (Hq / p.pack) * B;
+  p.out_rows = rows * (Hq / p.pack) * B;
+  p.part_rows = (int)(rows < p.block_rows ? rows : p.block_rows);
+  p.part_floats = (p.part_rows * (D + 2) + 3) / 4 * 4;
+  const int tiles = (Lk + 31) / 32;
+  int64_t n = 2 * (int64_t)cus / p.blocks;
+  if (n > (tiles + 7) / 8) n = (tiles + 7) / 8;
+  const size_t part = (size_t)p.blocks * p.part_floats * sizeof(float);
+  if (n > 1 && part * (size_t)n > scratch) n = (int64_t)(scratch / part);
+  p.splits = n > 1 ? (int)n : 1;
+  p.bytes = p.splits > 1 ? part * p.splits : 0;
+  return p;
+}
+
+// ---------------------------------------------------------------------------
 // the token-row kernels (prep.hip, adaln.hip)
 // ---------------------------------------------------------------------------
 

@@ -368,6 +368,52 @@ void head_norm_rope(const OperatorHandle& op, DispatchKeySet ks, Stack* stack) {
   c.give(std::move(q_out), std::move(k_out));
 }
 
+// masked_attn(q, k, v, softmax_scale, causal, softcap, bias?, doc_starts?, prefix_lens?, seqlen_k?, q_start?)
+void masked_attn(const OperatorHandle& op, DispatchKeySet ks, Stack* stack) {
+  Call c(op, stack);
+  const Tensor &q = c.tensor(0), &k = c.tensor(1), &v = c.tensor(2);
+  const auto dev = q.device();
+  const int type = dtype_of(q);
+  const bool causal = c[4].toBool();
+  bool ok = dev.is_cuda() && (type == WAN_BF16 || type == WAN_F16) && q.dim() == 4 &&
+            (q.size(3) == 64 || q.size(3) == 128) && heads4(q, q.scalar_type(), q.size(3), dev) &&
+            heads4(k, q.scalar_type(), q.size(3), dev) && heads4(v, q.scalar_type(), q.size(3), dev) &&
+            k.sizes() == v.sizes() && q.size(0) == k.size(0) && q.size(2) % k.size(2) == 0;
+  wan_attn_mask m{};
+  if (ok && c.has(6)) {
+    const Tensor& t = c.tensor(6);
+    ok = t.dim() == 2 && t.size(0) == q.size(2) && t.size(1) % 2 == 1 && small_int(t.size(1)) &&
+         vec(t, t.numel(), at::kFloat, dev);
+    if (ok) m.bias_reach = (int)(t.size(1) / 2);
+  }
+  if (ok && c.has(7)) {
+    const Tensor& t = c.tensor(7);
+    ok = t.dim() == 2 && t.size(0) == q.size(0) && t.size(1) > 0 && small_int(t.size(1)) && vec(t, t.numel(), at::kInt, dev);
+    if (ok) m.docs = (int)t.size(1);
+  }
+  if (ok && c.has(8)) {
+    const Tensor& t = c.tensor(8);
+    ok = causal && t.dim() == (m.docs ? 2 : 1) && t.size(0) == q.size(0) && (!m.docs || t.size(1) == m.docs) &&
+         vec(t, t.numel(), at::kInt, dev);
+  }
+  if (!ok || !lengths(c, 9, q.size(0), dev) || !lengths(c, 10, q.size(0), dev)) return to_python(op, ks, stack);
+  m.causal = causal;
+  m.softcap = c.real(5);
+  m.bias = static_cast<const float*>(c.ptr(6));
+  m.doc_starts = static_cast<const int32_t*>(c.ptr(7));
+  m.prefix_lens = static_cast<const int32_t*>(c.ptr(8));
+  m.seqlen_k = static_cast<const int32_t*>(c.ptr(9));
+  m.q_start = static_cast<const int32_t*>(c.ptr(10));
+  const int B = (int)q.size(0), Hq = (int)q.size(2), Hk = (int)k.size(2), Lq = (int)q.size(1), Lk = (int)k.size(1),
+            D = (int)q.size(3);
+  const Site s(q);
+  Tensor out = s.rows(q);
+  const Scratch ws(s, wan_masked_attn_workspace(B, Hq, Hk, Lq, Lk, D));
+  check("wan_masked_attn", wan_masked_attn(t4(q), t4(k), t4(v), t4(out), B, Hq, Hk, Lq, Lk, D, type, c.real(3), &m,
+                                           ws.ptr(), ws.n, s.stream()));
+  c.give(std::move(out));
+}
+
 // adaln(x, y?, e?, frames, gate_idx, shift_idx, scale_idx, ln_weight?, ln_bias?, eps, norm, e_mod?)
 void adaln(const OperatorHandle& op, DispatchKeySet ks, Stack* stack) {
   Call c(op, stack);
@@ -447,7 +493,7 @@ void linear(const OperatorHandle& op, DispatchKeySet ks, Stack* stack) {
   X("flash_self_attn", flash_self_attn) X("cross_attn", cross_attn) X("self_attn_fused", self_attn_fused) \
   X("self_attn_fused_sumsq", self_attn_fused_sumsq) X("cross_attn_fused", cross_attn_fused)         \
   X("flash_attn_qnorm", flash_attn_qnorm) X("rope", rope_op) X("rms_norm", rms_norm) X("rms_inv", rms_inv) \
-  X("head_norm_rope", head_norm_rope) X("adaln", adaln) X("qkv_proj_sumsq", qkv_proj_sumsq) X("linear", linear)
+  X("head_norm_rope", head_norm_rope) X("masked_attn", masked_attn) X("adaln", adaln) X("qkv_proj_sumsq", qkv_proj_sumsq) X("linear", linear)
 
 TORCH_LIBRARY_IMPL(wan_hip, CUDA, m) {
 #define WAN_IMPL(name, fn) m.impl(name, torch::CppFunction::makeFromBoxedFunction<&defined<&fn>>());

@@ -378,6 +378,75 @@ def _(q, k, gamma_q, gamma_k, eps, cos=None, sin=None, positions=None, interleav
     return q.new_empty(q.shape), k.new_empty(k.shape)
 
 
+# ─── attention under masks ────────────────────────────────────────────────────
+
+@torch.library.custom_op("wan_hip::masked_attn", mutates_args=())
+def masked_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, softmax_scale: float, causal: bool = False,
+                softcap: float = 0.0, bias: Optional[torch.Tensor] = None, doc_starts: Optional[torch.Tensor] = None,
+                prefix_lens: Optional[torch.Tensor] = None, seqlen_k: Optional[torch.Tensor] = None,
+                q_start: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of q [B, Lq, Hq, D] over k, v [B, Lk, Hk, D] (bf16 or fp16, D 64 or 128, Hq a multiple of
+    Hk) with the score changes and masks of wan_masked_attn:
+
+        p_i  = q_start[b] + i                    (default Lk - Lq + i: the last row is at the last key)
+        s_ij = softmax_scale q_i . k_j;  s = softcap tanh(s / softcap);  s += bias[h, clamp(j - p_i, -R, R) + R]
+
+    bias: fp32 [Hq, 2 R + 1].  Row i sees key j if j < seqlen_k[b] (default Lk); if j and p_i are of one
+    document, doc_starts [B, n] being the ascending first positions of the documents; and, if causal, if
+    j <= p_i or j is among the first prefix_lens [B] keys (with documents [B, n], of its document).  These are
+    int32.  A row that sees no key is zeros."""
+    fn = "masked_attn"
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        _check_heads(f"{fn}: {name}", t, (64, 128), (torch.bfloat16, torch.float16))
+    if k.shape != v.shape:
+        raise ValueError(f"{fn}: k {tuple(k.shape)} and v {tuple(v.shape)} differ")
+    if not (q.dtype == k.dtype == v.dtype) or not (q.device == k.device == v.device):
+        raise ValueError(f"{fn}: q, k, v are of different types or on different devices")
+    B, Lq, Hq, D = q.shape
+    Lk, Hk = k.shape[1:3]
+    if k.shape[0] != B or k.shape[3] != D or (Hq and (Hk == 0 or Hq % Hk)):
+        raise ValueError(f"{fn}: q {tuple(q.shape)} and k {tuple(k.shape)} disagree on batch, heads or head_dim")
+    reach = docs = 0
+    if bias is not None:
+        if bias.dim() != 2 or bias.shape[0] != Hq or bias.shape[1] % 2 != 1:
+            raise ValueError(f"{fn}: bias must be [{Hq}, 2 R + 1], got {tuple(bias.shape)}")
+        _check_vec(fn, "bias", bias, bias.numel(), torch.float32, q.device)
+        reach = bias.shape[1] // 2
+    if doc_starts is not None:
+        if doc_starts.dim() != 2 or doc_starts.shape[0] != B or doc_starts.shape[1] == 0:
+            raise ValueError(f"{fn}: doc_starts must be [{B}, n], got {tuple(doc_starts.shape)}")
+        docs = doc_starts.shape[1]
+        _check_vec(fn, "doc_starts", doc_starts, B * docs, torch.int32, q.device)
+    if prefix_lens is not None:
+        want = (B, docs) if docs else (B,)
+        if not causal or prefix_lens.shape != want:
+            raise ValueError(f"{fn}: prefix_lens go with causal and must be {list(want)}, got {tuple(prefix_lens.shape)}")
+        _check_vec(fn, "prefix_lens", prefix_lens, prefix_lens.numel(), torch.int32, q.device)
+    for name, t in (("seqlen_k", seqlen_k), ("q_start", q_start)):
+        if t is not None:
+            _check_vec(fn, name, t, B, torch.int32, q.device)
+    out = torch.empty((B, Lq, Hq, D), dtype=q.dtype, device=q.device)
+    lib = N.lib()
+
+    def ptr(t):
+        return None if t is None else t.data_ptr()
+    mask = N.WanAttnMask(int(causal), float(softcap), ptr(bias), reach, ptr(doc_starts), docs, ptr(prefix_lens),
+                         ptr(seqlen_k), ptr(q_start))
+    with torch.cuda.device(q.device):
+        n = lib.wan_masked_attn_workspace(B, Hq, Hk, Lq, Lk, D)
+        ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
+        N.check("wan_masked_attn", lib.wan_masked_attn(
+            N.tensor4(q), N.tensor4(k), N.tensor4(v), N.tensor4(out), B, Hq, Hk, Lq, Lk, D, _DTYPES[q.dtype],
+            float(softmax_scale), mask, ptr(ws), n, _stream(q.device)))
+    return out
+
+
+@masked_attn.register_fake
+def _(q, k, v, softmax_scale, causal=False, softcap=0.0, bias=None, doc_starts=None, prefix_lens=None, seqlen_k=None,
+      q_start=None):
+    return q.new_empty(q.shape)
+
+
 # ─── adaLN: the pointwise stages of a WanAttentionBlock ─────────────────────
 
 def _check_rows(fn: str, name: str, t: torch.Tensor, shape, device) -> None:
