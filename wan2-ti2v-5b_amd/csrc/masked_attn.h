@@ -16,8 +16,8 @@
 // V^T P^T without a shuffle.  Scores are kept in units of log2(e): the largest finite bias stays finite.
 //
 // A masked key's weight is an exact 0, and 0 times a NaN or an infinity in its v row must not reach the
-// output: tiles that need a mask are looked over, and where such a value is found their products are formed
-// one by one for the keys that a row sees (exact_pv).
+// output: tiles that need a mask are looked over, and where such a value is found it goes to the rows alone
+// that see it (exact_pv).
 
 // ---------------------------------------------------------------------------
 // element types
@@ -168,14 +168,13 @@ __device__ __forceinline__ int rows_max(int v) {
   return __builtin_amdgcn_readfirstlane(v);
 }
 
-// Which rows a block number stands for.
-struct MaskedBlock {
-  int b, h0, hk, rb;      // sample, first of the P query heads, their k/v head, block of rows
-  __device__ __forceinline__ MaskedBlock(const MaskedArgs& a, int id, int blocks) {
-    const int unit = id / blocks, per = a.Hq / a.pack;
-    const int sample = unit / per, first = (unit - sample * per) * a.pack;
-    rb = uniform(id - unit * blocks);
-    b = uniform(sample);
+// The sample and heads of a unit.  The samples vary fastest: units that run together are then long and
+// short ones alike.
+struct MaskedUnit {
+  int b, h0, hk;          // sample, first of the P query heads, their k/v head
+  __device__ __forceinline__ MaskedUnit(const MaskedArgs& a, int unit) {
+    const int group = unit / a.B, first = group * a.pack;
+    b = uniform(unit - group * a.B);
     h0 = uniform(first);
     hk = uniform(first / (a.Hq / a.Hk));
   }
@@ -189,8 +188,8 @@ struct TileRange {
   int first, end;
   __device__ __forceinline__ TileRange(int t0, int n, int part, int parts) {
     const int each = n / parts, over = n - each * parts;
-    first = MaskedBlock::uniform(t0 + each * part + min(part, over));
-    end = MaskedBlock::uniform(t0 + each * (part + 1) + min(part + 1, over));
+    first = MaskedUnit::uniform(t0 + each * part + min(part, over));
+    end = MaskedUnit::uniform(t0 + each * (part + 1) + min(part + 1, over));
   }
 };
 
@@ -285,43 +284,13 @@ template <typename T, int HD, int KEYS>
 __device__ __forceinline__ bool tile_not_finite(const bf16* Vt, int lane) {
   constexpr uint32_t M = Elem<T>::kExpBits * 0x10001u;
   u16x2 top = {0, 0};
-#pragma unroll
+#pragma unroll 2        // (few registers: the kernels hold their accumulators here)
   for (int i = 0; i < KEYS * HD / 512; ++i) {
     const u32x4 w = *reinterpret_cast<const u32x4*>(Vt + i * 512 + lane * 8);
 #pragma unroll
     for (int j = 0; j < 4; ++j) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, w[j] & M));
   }
   return __builtin_amdgcn_ballot_w64(top[0] == Elem<T>::kExpBits || top[1] == Elem<T>::kExpBits) != 0;
-}
-
-// O^T += V^T P^T of 16 keys, product by product, of the keys from key0 on that this lane's row sees.
-// `buf`: 1 KB of this wave's.
-template <typename T, int HD>
-__device__ __forceinline__ void exact_pv(f32x16 (&o)[HD / 32], typename Elem<T>::x8 pb, const bf16* Vt, int row0, int key0,
-                                         const MaskedRow& m, T* buf, int lane) {
-  typedef typename Elem<T>::x4 X4;
-  const int n32 = lane & 31, hh = lane >> 5;
-  // this lane's weights are of keys 4 hh .. +3 and 8 + 4 hh .. +3
-  *reinterpret_cast<X4*>(buf + n32 * 16 + 4 * hh) = X4{pb[0], pb[1], pb[2], pb[3]};
-  *reinterpret_cast<X4*>(buf + n32 * 16 + 8 + 4 * hh) = X4{pb[4], pb[5], pb[6], pb[7]};
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-#pragma nounroll
-  for (int kk = 0; kk < 16; ++kk) {
-    const float p = (float)buf[n32 * 16 + kk];
-    const bool sees = key0 + kk >= m.lo && key0 + kk < m.hi;
-    const T* row = reinterpret_cast<const T*>(Vt) + (row0 + kk) * HD;
-    const int x = mv_swz<HD>(row0 + kk);
-#pragma unroll
-    for (int md = 0; md < HD / 32; ++md)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const X4 v = *reinterpret_cast<const X4*>(row + (((4 * md + g) ^ x) << 3) + 4 * hh);
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          o[md][4 * g + e] = sees ? fmaf(p, (float)v[e], o[md][4 * g + e]) : o[md][4 * g + e];
-      }
-  }
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 }
 
 // What a lane reads of the tiles, and its Q fragments.
@@ -356,6 +325,46 @@ struct MaskedOperands {
   }
 };
 
+// O^T += V^T P^T of a tile of 16 N keys from key kt on that holds NaNs or infinities, some of them perhaps of
+// keys that a row does not see.  Their products are left out (v as 0); then each row gets the infinities of the
+// keys that it sees: their number is the product of v's bad places (+inf 1, -inf 128, NaN both) with the keys
+// that the row sees (1 or 0), which is exact.
+template <typename T, int HD, int N>
+__device__ __forceinline__ void exact_pv(const MaskedOperands<T, HD>& op, f32x16 (&o)[HD / 32],
+                                         const typename Elem<T>::x8 (&pb)[N], const bf16* Vt, int kt, const MaskedRow& m,
+                                         int hh) {
+  typedef typename Elem<T>::x8 X8;
+  typedef unsigned short U8 __attribute__((ext_vector_type(8)));
+  constexpr unsigned short M = Elem<T>::kExpBits;
+#pragma unroll
+  for (int md = 0; md < HD / 32; ++md) {
+    f32x16 count = {};
+#pragma unroll
+    for (int ksp = 0; ksp < N; ++ksp) {
+      const U8 v = __builtin_bit_cast(U8, op.v_frag(Vt, ksp, md));
+      U8 good;
+      X8 bad, sees;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const bool is_bad = (v[e] & M) == M, nan = (v[e] & 0x7fff) != M;
+        good[e] = is_bad ? 0 : v[e];
+        bad[e] = (T)(!is_bad ? 0.f : nan ? 129.f : v[e] & 0x8000 ? 128.f : 1.f);
+        const int key = kt + 16 * ksp + 4 * hh + (e & 3) + 8 * (e >> 2);
+        sees[e] = (T)(key >= m.lo && key < m.hi ? 1.f : 0.f);
+      }
+      o[md] = Elem<T>::mfma(__builtin_bit_cast(X8, good), pb[ksp], o[md]);
+      count = Elem<T>::mfma(bad, sees, count);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const float down = floorf(count[r] * (1.f / 128.f));
+      o[md][r] += count[r] - 128.f * down > 0.f ? INFINITY : 0.f;
+      o[md][r] += down > 0.f ? -INFINITY : 0.f;
+    }
+  }
+}
+
 // The interval test of the 16 keys that a lane's accumulator holds, from key kt on: masked scores become -inf.
 __device__ __forceinline__ void mask_scores(f32x16& s, int kt, int hh, const MaskedRow& m) {
   const uint32_t n = (uint32_t)(m.hi - m.lo);
@@ -373,72 +382,79 @@ __device__ __forceinline__ float max16(const f32x16& s) {
 }
 
 // ---------------------------------------------------------------------------
-// few rows: 32 rows a workgroup, its four waves on every fourth tile of 32 keys
+// 32 rows on tiles of 32 keys, by one wave alone
 // ---------------------------------------------------------------------------
 
-constexpr int kStepWaves = 4, kStepKeys = 32;
-constexpr int kStepWindow = 1200;       // bias entries of a wave
+constexpr int kWaveKeys = 32;
 
-template <typename T, int HD, bool CAP, bool BIAS>
-__global__ __launch_bounds__(kStepWaves * 64, 1) void masked_step_kernel(const MaskedArgs a) {
+// The rows of a wave: this lane's query and head, its interval, and what any and every row of the wave sees.
+struct WaveRows {
+  int i, g;
+  MaskedRow m;
+  int first, end, all_lo, all_hi;
+  // rows row0 .. row0 + 31 of a unit; those past the last one repeat it (they are not stored)
+  __device__ __forceinline__ WaveRows(const MaskedArgs& a, int b, int row0, int rows, int lane) {
+    const int r = min(row0 + (lane & 31), rows - 1);
+    i = r / a.pack;
+    g = r - i * a.pack;
+    m = masked_row(a, b, i);
+    const bool some = m.lo < m.hi;
+    first = rows_min(some ? m.lo : 0x7fffffff);
+    end = rows_max(m.hi);
+    all_lo = rows_max(m.lo);
+    all_hi = rows_min(m.hi);
+  }
+};
+
+// The tiles t, t + stride, ... < tb through SLOTS slots of k and v tiles at `tiles`, all of it this wave's
+// own: copies of the next SLOTS - 1 tiles in flight, no barrier.  `window`: kept bias entries (`floats`).
+// Leaves O unnormalised, its reference point and this lane's sum.
+template <typename T, int HD, bool CAP, bool BIAS, int SLOTS>
+__device__ __forceinline__ void attend_wave(const MaskedArgs& a, const MaskedUnit& u, const WaveRows& w, int t, int tb,
+                                            int stride, bf16* tiles, float* window, int floats, int lane,
+                                            f32x16 (&o)[HD / 32], float& m_run, float& l_run) {
   typedef typename Elem<T>::x8 X8;
-  constexpr int kTile = kStepKeys * HD;       // elements
-  __shared__ __attribute__((aligned(1024))) bf16 tiles[kStepWaves][2][2][kTile];     // [wave][slot][k, v]
-  __shared__ __attribute__((aligned(16))) T exact_buf[kStepWaves][32 * 16];
-  __shared__ float window[kStepWaves][BIAS ? kStepWindow : 1];
-
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int n32 = lane & 31, hh = lane >> 5;
-  const int rows = a.Lq * a.pack, blocks = (rows + 31) / 32;
-  const int slot_id = blockIdx.x / a.splits, part = blockIdx.x - slot_id * a.splits;
-  const MaskedBlock blk(a, slot_id, blocks);
-  // (rows past the last one repeat it; they are not stored)
-  const int r = min(blk.rb * 32 + n32, rows - 1), i = r / a.pack, g = r - i * a.pack;
-  const MaskedRow m = masked_row(a, blk.b, i);
-
-  // this part's tiles
-  const bool some = m.lo < m.hi;
-  const int first = rows_min(some ? m.lo : 0x7fffffff), end = rows_max(m.hi);
-  const int all_lo = rows_max(m.lo), all_hi = rows_min(m.hi);     // what every row sees: [all_lo, all_hi)
-  const int t0 = first / kStepKeys;
-  const TileRange range(t0, first < end ? (end - 1) / kStepKeys + 1 - t0 : 0, part, a.splits);
-  const int tb = range.end;
-
-  MaskedCopy<HD, kStepKeys, 1, false> kc;
-  MaskedCopy<HD, kStepKeys, 1, true> vc;
-  kc.init(static_cast<const T*>(a.k.ptr) + blk.b * a.k.sb + blk.hk * a.k.sh, a.k.st, 0, lane);
-  vc.init(static_cast<const T*>(a.v.ptr) + blk.b * a.v.sb + blk.hk * a.v.sh, a.v.st, 0, lane);
+  constexpr int kTile = kWaveKeys * HD;       // elements
+  const int hh = lane >> 5;
+  MaskedCopy<HD, kWaveKeys, 1, false> kc;
+  MaskedCopy<HD, kWaveKeys, 1, true> vc;
+  kc.init(static_cast<const T*>(a.k.ptr) + u.b * a.k.sb + u.hk * a.k.sh, a.k.st, 0, lane);
+  vc.init(static_cast<const T*>(a.v.ptr) + u.b * a.v.sb + u.hk * a.v.sh, a.v.st, 0, lane);
   auto issue = [&](int t, int slot) {
-    kc.issue(t, a.Lk, tiles[wave][slot][0], 0, lane);
-    vc.issue(t, a.Lk, tiles[wave][slot][1], 0, lane);
+    kc.issue(t, a.Lk, tiles + slot * (2 * kTile), 0, lane);
+    vc.issue(t, a.Lk, tiles + slot * (2 * kTile) + kTile, 0, lane);
   };
-  int t = range.first + wave;
-  if (t < tb) issue(t, 0);
-  if (t + kStepWaves < tb) issue(t + kStepWaves, 1);
+#pragma unroll
+  for (int n = 0; n < SLOTS; ++n)
+    if (t + n * stride < tb) issue(t + n * stride, n);
 
   MaskedOperands<T, HD> op;
-  op.init(static_cast<const T*>(a.q.ptr) + blk.b * a.q.sb + (int64_t)i * a.q.st + (blk.h0 + g) * a.q.sh, lane);
+  op.init(static_cast<const T*>(a.q.ptr) + u.b * a.q.sb + (int64_t)w.i * a.q.st + (u.h0 + w.g) * a.q.sh, lane);
   ScoreMap<CAP, BIAS> map;
   map.init(a);
   BiasWindow win;
-  if (BIAS) win.init(kStepWindow, a.pack);
-  const int p_max = rows_max(m.p), p_min = rows_min(m.p);
-
-  f32x16 o[HD / 32];
+  int p_max = 0, p_min = 0;
+  if constexpr (BIAS) {
+    win.init(floats, a.pack);
+    p_max = rows_max(w.m.p);
+    p_min = rows_min(w.m.p);
+  }
 #pragma unroll
   for (int md = 0; md < HD / 32; ++md) o[md] = f32x16{};
-  float m_run = -FLT_MAX, l_run = 0.f;
+  m_run = -FLT_MAX;
+  l_run = 0.f;
 
-  for (int slot = 0; t < tb; t += kStepWaves, slot ^= 1) {
-    const int kt = t * kStepKeys;
-    const bf16 *Kt = tiles[wave][slot][0], *Vt = tiles[wave][slot][1];
-    if (BIAS && !win.holds(kt - p_max, kt + kStepKeys - 1 - p_min)) {
-      win.load(a, blk.h0, kt - p_max, (int64_t)(tb - t) * kStepKeys + (p_max - p_min), window[wave], lane, 64);
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  for (int slot = 0; t < tb; t += stride, slot = SLOTS == 1 ? 0 : slot ^ 1) {
+    const int kt = t * kWaveKeys;
+    const bf16 *Kt = tiles + slot * (2 * kTile), *Vt = Kt + kTile;
+    if constexpr (BIAS) {
+      if (!win.holds(kt - p_max, kt + kWaveKeys - 1 - p_min)) {
+        win.load(a, u.h0, kt - p_max, (int64_t)(tb - t) * kWaveKeys + (p_max - p_min), window, lane, 64);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      }
     }
     // this tile has landed; the next one's copies stay in flight
-    if (t + kStepWaves < tb)
+    if (SLOTS > 1 && t + stride < tb)
       asm volatile("s_waitcnt vmcnt(%0)" :: "i"(2 * decltype(kc)::kPer) : "memory");
     else
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -448,12 +464,12 @@ __global__ __launch_bounds__(kStepWaves * 64, 1) void masked_step_kernel(const M
     for (int ks = 0; ks < HD / 16; ++ks) s = Elem<T>::mfma(op.k_frag(Kt, ks, 0), op.qf[ks], s);
     map.map(s);
     if constexpr (BIAS) {
-      const float* w = window[wave] + g * win.per + (kt + 4 * hh - m.p - win.w0);
+      const float* e0 = window + w.g * win.per + (kt + 4 * hh - w.m.p - win.w0);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) s[e] += w[8 * (e >> 2) + (e & 3)];
+      for (int e = 0; e < 16; ++e) s[e] += e0[8 * (e >> 2) + (e & 3)];
     }
-    const bool masked = kt < all_lo || kt + kStepKeys > all_hi;
-    if (masked) mask_scores(s, kt, hh, m);
+    const bool masked = kt < w.all_lo || kt + kWaveKeys > w.all_hi;
+    if (masked) mask_scores(s, kt, hh, w.m);
 
     const float m_new = fmaxf(m_run, map.top(pair_max(max16(s))));
     if (__builtin_amdgcn_ballot_w64(m_new > m_run) != 0) {
@@ -466,14 +482,13 @@ __global__ __launch_bounds__(kStepWaves * 64, 1) void masked_step_kernel(const M
     X8 pb[2];
 #pragma unroll
     for (int e = 0; e < 16; e += 2) {
-      typename Elem<T>::x2 w = {(T)map.weight(s[e], m_run), (T)map.weight(s[e + 1], m_run)};
-      pb[e >> 3][e & 7] = w[0];
-      pb[e >> 3][(e & 7) + 1] = w[1];
-      l_run = Elem<T>::add2(w, l_run);      // the sum of the rounded weights that the products use
+      const typename Elem<T>::x2 p = {(T)map.weight(s[e], m_run), (T)map.weight(s[e + 1], m_run)};
+      pb[e >> 3][e & 7] = p[0];
+      pb[e >> 3][(e & 7) + 1] = p[1];
+      l_run = Elem<T>::add2(p, l_run);      // the sum of the rounded weights that the products use
     }
-    if (masked && tile_not_finite<T, HD, kStepKeys>(Vt, lane)) {
-#pragma unroll
-      for (int ksp = 0; ksp < 2; ++ksp) exact_pv<T, HD>(o, pb[ksp], Vt, 16 * ksp, kt + 16 * ksp, m, exact_buf[wave], lane);
+    if (masked && tile_not_finite<T, HD, kWaveKeys>(Vt, lane)) {
+      exact_pv<T, HD>(op, o, pb, Vt, kt, w.m, hh);
     } else {
 #pragma unroll
       for (int ksp = 0; ksp < 2; ++ksp)
@@ -482,15 +497,46 @@ __global__ __launch_bounds__(kStepWaves * 64, 1) void masked_step_kernel(const M
     }
     // every read of this slot has returned before it is filled again
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    if (t + 2 * kStepWaves < tb) issue(t + 2 * kStepWaves, slot);
+    if (t + SLOTS * stride < tb) issue(t + SLOTS * stride, slot);
   }
+}
+
+// ---------------------------------------------------------------------------
+// few rows: 32 rows a workgroup, its four waves on every fourth tile
+// ---------------------------------------------------------------------------
+
+constexpr int kStepWaves = 4;
+constexpr int kStepWindow = 1200;       // bias entries of a wave
+
+template <typename T, int HD, bool CAP, bool BIAS>
+__global__ __launch_bounds__(kStepWaves * 64, 1) void masked_step_kernel(const MaskedArgs a) {
+  typedef typename Elem<T>::x8 X8;
+  constexpr int kTiles = 4 * kWaveKeys * HD;         // a wave's two slots of k and v, elements
+  __shared__ __attribute__((aligned(1024))) bf16 tiles[kStepWaves][kTiles];
+  __shared__ float window[kStepWaves][BIAS ? kStepWindow : 1];
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n32 = lane & 31, hh = lane >> 5;
+  const int rows = a.Lq * a.pack, blocks = (rows + 31) / 32;
+  const int block = blockIdx.x / a.splits, part = blockIdx.x - block * a.splits;
+  const MaskedUnit blk(a, block / blocks);
+  const int row0 = block % blocks * 32;
+  const WaveRows w(a, blk.b, row0, rows, lane);
+  const int t0 = w.first / kWaveKeys;
+  const TileRange range(t0, w.first < w.end ? (w.end - 1) / kWaveKeys + 1 - t0 : 0, part, a.splits);
+
+  f32x16 o[HD / 32];
+  float m_run, l_run;
+  attend_wave<T, HD, CAP, BIAS, 2>(a, blk, w, range.first + wave, range.end, kStepWaves, tiles[wave], window[wave],
+                                   kStepWindow, lane, o, m_run, l_run);
   l_run = pair_sum(l_run);
 
   // The four waves' results through LDS: O [32][HD + 4], then each row's weights.
   constexpr int kRow = HD + 4;
   static_assert(kStepWaves * 32 * (kRow + 2) * 4 <= (int)sizeof(tiles), "the tiles hold the waves' results");
   __syncthreads();
-  float* const all = reinterpret_cast<float*>(&tiles[0][0][0][0]);
+  float* const all = reinterpret_cast<float*>(&tiles[0][0]);
   float* const mine = all + wave * (32 * kRow);
   float* const stat = all + kStepWaves * (32 * kRow);       // m [4][32], l [4][32]
 #pragma unroll
@@ -504,19 +550,19 @@ __global__ __launch_bounds__(kStepWaves * 64, 1) void masked_step_kernel(const M
     stat[(kStepWaves + wave) * 32 + n32] = l_run;
   }
   __syncthreads();
-  const int held = min(rows - blk.rb * 32, 32);             // rows of this block
+  const int held = min(rows - row0, 32);             // rows of this block
   for (int x = threadIdx.x; x < held * (HD / 8); x += kStepWaves * 64) {
     const int row = x / (HD / 8), c = x - row * (HD / 8);
     float top = stat[row], l = 0.f;
 #pragma unroll
-    for (int w = 1; w < kStepWaves; ++w) top = fmaxf(top, stat[w * 32 + row]);
+    for (int n = 1; n < kStepWaves; ++n) top = fmaxf(top, stat[n * 32 + row]);
     float v[8] = {};
 #pragma unroll
-    for (int w = 0; w < kStepWaves; ++w) {
-      const float f = fast_exp2(stat[w * 32 + row] - top);
-      l += f * stat[(kStepWaves + w) * 32 + row];
+    for (int n = 0; n < kStepWaves; ++n) {
+      const float f = fast_exp2(stat[n * 32 + row] - top);
+      l += f * stat[(kStepWaves + n) * 32 + row];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = fmaf(f, all[w * (32 * kRow) + row * kRow + 8 * c + e], v[e]);
+      for (int e = 0; e < 8; ++e) v[e] = fmaf(f, all[n * (32 * kRow) + row * kRow + 8 * c + e], v[e]);
     }
     if (a.splits > 1) {
       float* p = a.part + (int64_t)blockIdx.x * a.part_floats + row * HD + 8 * c;
@@ -529,13 +575,340 @@ __global__ __launch_bounds__(kStepWaves * 64, 1) void masked_step_kernel(const M
       }
     } else {
       const float inv = l == 0.f ? 0.f : 1.f / l;
-      const int rr = blk.rb * 32 + row, qi = rr / a.pack;
+      const int rr = row0 + row, qi = rr / a.pack;
       X8 y;
 #pragma unroll
       for (int e = 0; e < 8; ++e) y[e] = (T)(v[e] * inv);
       *reinterpret_cast<X8*>(static_cast<T*>(a.o) + blk.b * a.o_sb + (int64_t)qi * a.o_st +
                              (blk.h0 + rr - qi * a.pack) * a.o_sh + 8 * c) = y;
     }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// many rows: 256 rows a workgroup, 32 a wave, on tiles of 64 keys that all waves share
+// ---------------------------------------------------------------------------
+
+constexpr int kBlockWaves = kAttnWaves, kBlockKeys = kTileKeys;
+constexpr int kBlockWindow = 8128;      // bias entries of a workgroup
+
+// The arithmetic of a wave's 32 rows on a tile of 64 keys (scores c0: keys 0 .. 31, c1: 32 .. 63).
+template <typename T, int HD, bool CAP, bool BIAS>
+struct BlockCore {
+  typedef typename Elem<T>::x8 X8;
+  typedef typename Elem<T>::x2 X2;
+  // A lane's sum of a tile's weights that makes the wave take a new reference point: with less, every
+  // weight fits the type, and a reference point below the running max cancels in O / l.
+  static constexpr float kBound = sizeof(X8) == 16 && Elem<T>::kExpBits == 0x7c00 ? 32768.f : kSumBound;
+  static constexpr int kSteps = HD / 16, kEach = 16 / kSteps;    // MFMA steps, scores of a half in each
+
+  MaskedOperands<T, HD> op;
+  ScoreMap<CAP, BIAS> map;
+  f32x16 o[HD / 32];
+  float m_run, l_run;
+
+  __device__ __forceinline__ void reset() {
+#pragma unroll
+    for (int md = 0; md < HD / 32; ++md) o[md] = f32x16{};
+    m_run = -FLT_MAX;
+    l_run = 0.f;
+  }
+
+  __device__ __forceinline__ void qk(const bf16* Kt, f32x16& s0, f32x16& s1) const {
+    s0 = f32x16{};
+    s1 = f32x16{};
+#pragma unroll
+    for (int ks = 0; ks < kSteps; ++ks) {
+      s0 = Elem<T>::mfma(op.k_frag(Kt, ks, 0), op.qf[ks], s0);
+      s1 = Elem<T>::mfma(op.k_frag(Kt, ks, 32), op.qf[ks], s1);
+    }
+  }
+
+  __device__ __forceinline__ void weigh(const f32x16& c, int r, X8 pb[2], float& acc) const {
+    const X2 w = {(T)map.weight(c[r], m_run), (T)map.weight(c[r + 1], m_run)};
+    pb[r >> 3][r & 7] = w[0];
+    pb[r >> 3][(r & 7) + 1] = w[1];
+    acc = Elem<T>::add2(w, acc);
+  }
+
+  // The weights of a tile and this lane's sum of them (of the rounded values that the products use), eight
+  // exponentials in flight at most.
+  __device__ __forceinline__ float exp_tile(const f32x16& c0, const f32x16& c1, X8 pb[4]) const {
+    float acc[2] = {0.f, 0.f};
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int r = 0; r < 16; r += 2) {
+        weigh(h == 0 ? c0 : c1, r, pb + 2 * h, acc[h]);
+        if ((r & 7) == 6) __builtin_amdgcn_sched_barrier(0);
+      }
+    return acc[0] + acc[1];
+  }
+
+  // The same with the MFMAs of the next tile's scores in between, k fragments read one step ahead.
+  __device__ __forceinline__ float qk_exp(const bf16* Kt, f32x16& n0, f32x16& n1, const f32x16& c0, const f32x16& c1,
+                                          X8 pb[4]) const {
+    float acc0 = 0.f, acc1 = 0.f;
+    X8 a0 = op.k_frag(Kt, 0, 0), a1 = op.k_frag(Kt, 0, 32);
+#pragma unroll
+    for (int ks = 0; ks < kSteps; ++ks) {
+      X8 b0, b1;
+      if (ks < kSteps - 1) {
+        b0 = op.k_frag(Kt, ks + 1, 0);
+        b1 = op.k_frag(Kt, ks + 1, 32);
+      }
+      n0 = Elem<T>::mfma(a0, op.qf[ks], ks == 0 ? f32x16{} : n0);
+      n1 = Elem<T>::mfma(a1, op.qf[ks], ks == 0 ? f32x16{} : n1);
+#pragma unroll
+      for (int r = kEach * ks; r < kEach * (ks + 1); r += 2) {
+        weigh(c0, r, pb, acc0);
+        weigh(c1, r, pb + 2, acc1);
+      }
+      if (ks < kSteps - 1) {
+        a0 = b0;
+        a1 = b1;
+      }
+    }
+    return acc0 + acc1;
+  }
+
+  __device__ __forceinline__ float tile_top(const f32x16& c0, const f32x16& c1) const {
+    return map.top(pair_max(fmaxf(max16(c0), max16(c1))));
+  }
+
+  // Takes a tile's sum of weights rs; a row whose sum passes the bound (or is inf or NaN) goes over to the tile's
+  // exact max, rescales and weighs again, with the wave's other rows as they were: no row's bits depend on
+  // what rows beside it hold.
+  __device__ __forceinline__ void finish(const f32x16& c0, const f32x16& c1, float rs, X8 pb[4]) {
+    const bool over = !(rs <= kBound);
+    if (__builtin_amdgcn_ballot_w64(over) != 0) {
+      const float top = tile_top(c0, c1);
+      const float m_new = pair_max(over ? 1.f : 0.f) > 0.f ? fmaxf(m_run, top) : m_run;
+      const float alpha = fast_exp2(m_run - m_new);
+      m_run = m_new;
+      l_run *= alpha;
+#pragma unroll
+      for (int md = 0; md < HD / 32; ++md) o[md] *= alpha;
+      rs = exp_tile(c0, c1, pb);
+    }
+    l_run += rs;
+  }
+
+  // O^T += V^T P^T, v fragments read one MFMA ahead
+  __device__ __forceinline__ void pv(const X8 pb[4], const bf16* Vt) {
+    constexpr int MD = HD / 32;
+    X8 cur = op.v_frag(Vt, 0, 0);
+#pragma unroll
+    for (int i = 0; i < 4 * MD; ++i) {
+      X8 nxt;
+      if (i < 4 * MD - 1) nxt = op.v_frag(Vt, (i + 1) / MD, (i + 1) % MD);
+      o[i % MD] = Elem<T>::mfma(cur, pb[i / MD], o[i % MD]);
+      if (i < 4 * MD - 1) cur = nxt;
+    }
+  }
+};
+
+template <typename T, int HD, bool CAP, bool BIAS>
+__global__ __launch_bounds__(kBlockWaves * 64, 2) void masked_block_kernel(const MaskedArgs a) {
+  typedef typename Elem<T>::x8 X8;
+  typedef typename Elem<T>::x4 X4;
+  constexpr int BM = kBlockWaves * 32, BK = kBlockKeys, kTile = BK * HD;
+  // Rings of four k and v tiles and a barrier every second tile, as in the unmasked kernel: an even step
+  // issues the copies of the next pair of tiles, the odd one waits for them.
+  __shared__ __attribute__((aligned(1024))) bf16 k_lds[4][kTile];
+  __shared__ __attribute__((aligned(1024))) bf16 v_lds[4][kTile];
+  __shared__ float window[BIAS ? kBlockWindow : 1];
+  __shared__ int ends[2][kBlockWaves];
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n32 = lane & 31, hh = lane >> 5;
+  const int rows = a.Lq * a.pack, blocks = (rows + BM - 1) / BM;
+  // Each XCD runs contiguous numbers: the blocks of one unit and part share k and v in its L2.  The last rows
+  // come first, under a causal mask they see the most keys.
+  const int id = xcd_remap(blockIdx.x, gridDim.x);
+  const int up = id / blocks, unit = up / a.splits, part = up - unit * a.splits;
+  const int row0 = MaskedUnit::uniform((blocks - 1 - (id - up * blocks)) * BM);
+  const MaskedUnit blk(a, unit);
+  const bool live = row0 + wave * 32 < rows;      // (a wave without rows copies its share and meets the barriers)
+  WaveRows w(a, blk.b, row0 + wave * 32, rows, lane);
+  if (!live) {
+    w.first = 0x7fffffff;
+    w.end = 0;
+  }
+  // the tiles that any row of the workgroup sees keys of, this part of them
+  if (lane == 0) {
+    ends[0][wave] = w.first;
+    ends[1][wave] = w.end;
+  }
+  __syncthreads();
+  int first = ends[0][0], end = ends[1][0];
+#pragma unroll
+  for (int n = 1; n < kBlockWaves; ++n) {
+    first = min(first, ends[0][n]);
+    end = max(end, ends[1][n]);
+  }
+  const TileRange range(first / BK, first < end ? (end - 1) / BK + 1 - first / BK : 0, part, a.splits);
+  const int nt = range.end - range.first;
+
+  BlockCore<T, HD, CAP, BIAS> c;
+  bool bad = false;       // a tile that needed a mask held a NaN or an infinity in v
+  c.reset();
+  c.map.init(a);
+  if (nt > 0) {
+    MaskedCopy<HD, BK, kBlockWaves, false> kc;
+    MaskedCopy<HD, BK, kBlockWaves, true> vc;
+    kc.init(static_cast<const T*>(a.k.ptr) + blk.b * a.k.sb + blk.hk * a.k.sh, a.k.st, wave, lane);
+    vc.init(static_cast<const T*>(a.v.ptr) + blk.b * a.v.sb + blk.hk * a.v.sh, a.v.st, wave, lane);
+    auto copy_k = [&](int u) {
+      if (u < nt) kc.issue(range.first + u, a.Lk, k_lds[u & 3], wave, lane);
+    };
+    auto copy_v = [&](int u) {
+      if (u < nt) vc.issue(range.first + u, a.Lk, v_lds[u & 3], wave, lane);
+    };
+    copy_k(0);
+    copy_v(0);
+    copy_k(1);
+    copy_v(1);
+    copy_k(2);
+    c.op.init(static_cast<const T*>(a.q.ptr) + blk.b * a.q.sb + (int64_t)w.i * a.q.st + (blk.h0 + w.g) * a.q.sh, lane);
+
+    BiasWindow win;
+    int p_first = 0, p_last = 0;       // positions of the workgroup's rows
+    if constexpr (BIAS) {
+      win.init(kBlockWindow, a.pack);
+      const int at = MaskedUnit::uniform(w.m.p - w.i);
+      p_first = at + row0 / a.pack;
+      p_last = at + (min(row0 + BM, rows) - 1) / a.pack;
+    }
+    // whether the wave's rows see any key of tile u
+    auto seen = [&](int u) {
+      const int kt = (range.first + u) * BK;
+      return u < nt && kt < w.end && kt + BK > w.first;
+    };
+    bool fresh = true;
+    auto step = [&](int u, f32x16& c0, f32x16& c1, f32x16& n0, f32x16& n1) {
+      const int kt = (range.first + u) * BK;
+      if constexpr (BIAS) {
+        if (!win.holds(kt - p_last, kt + BK - 1 - p_first)) {
+          __syncthreads();
+          win.load(a, blk.h0, kt - p_last, (int64_t)(nt - u) * BK + (p_last - p_first), window, threadIdx.x,
+                   kBlockWaves * 64);
+          __syncthreads();
+        }
+      }
+      const bool here = seen(u), next = seen(u + 1);
+      const bool masked = here && (kt < w.all_lo || kt + BK > w.all_hi);
+      const bf16 *Kn = k_lds[(u + 1) & 3], *Vt = v_lds[u & 3];
+      X8 pb[4];
+      if (here) {
+        c.map.map(c0);
+        c.map.map(c1);
+        if constexpr (BIAS) {
+          const float* e0 = window + w.g * win.per + (kt + 4 * hh - w.m.p - win.w0);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            c0[e] += e0[8 * (e >> 2) + (e & 3)];
+            c1[e] += e0[32 + 8 * (e >> 2) + (e & 3)];
+          }
+        }
+        if (masked) {
+          mask_scores(c0, kt, hh, w.m);
+          mask_scores(c1, kt + 32, hh, w.m);
+        }
+        if (fresh) {
+          c.m_run = fmaxf(-FLT_MAX, c.tile_top(c0, c1));
+          fresh = false;
+        }
+        const float rs = next ? c.qk_exp(Kn, n0, n1, c0, c1, pb) : c.exp_tile(c0, c1, pb);
+        c.finish(c0, c1, rs, pb);
+      } else if (next) {
+        c.qk(Kn, n0, n1);
+      }
+      if ((u & 1) == 0) {
+        copy_k(u + 3);
+        copy_k(u + 4);
+        copy_v(u + 2);
+        copy_v(u + 3);
+      }
+      if (here) {
+        if (masked) bad = bad || tile_not_finite<T, HD, BK>(Vt, lane);
+        c.pv(pb, Vt);
+      }
+      if (u & 1) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+      }
+    };
+
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    f32x16 sa0, sa1, sb0, sb1;
+    if (seen(0)) c.qk(k_lds[0], sa0, sa1);
+    __syncthreads();      // every wave is done with tile 0 of k before it is overwritten
+    for (int u = 0; u < nt; u += 2) {
+      step(u, sa0, sa1, sb0, sb1);
+      if (u + 1 < nt) step(u + 1, sb0, sb1, sa0, sa1);
+    }
+    __syncthreads();      // ... and with the last tiles before the output is staged over them
+  }
+  if (!live) return;
+  // This wave's share of the rings, from here on.
+  bf16* const share = wave < 4 ? k_lds[wave] : v_lds[wave - 4];
+  // Such a value may have reached rows that do not see it: the wave's rows once more, by itself.  (Told apart in
+  // the loop above, the second way to form O left it too few registers: 40 were spilled in every tile.)
+  if (bad)
+    attend_wave<T, HD, CAP, BIAS, 1>(a, blk, w, max(range.first * (BK / kWaveKeys), w.first / kWaveKeys),
+                                     min(range.end * (BK / kWaveKeys), (w.end - 1) / kWaveKeys + 1), 1,
+                                     share, window + wave * (kBlockWindow / kBlockWaves), kBlockWindow / kBlockWaves,
+                                     lane, c.o, c.m_run, c.l_run);
+  const float l = pair_sum(c.l_run);
+  const int held = min(rows - row0 - wave * 32, 32);        // rows of this wave
+  if (a.splits > 1) {
+    const int block = unit * blocks + row0 / BM, at = wave * 32 + n32;
+    float* p = a.part + ((int64_t)block * a.splits + part) * a.part_floats;
+    if (n32 < held) {
+#pragma unroll
+      for (int md = 0; md < HD / 32; ++md)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          *reinterpret_cast<f32x4*>(p + at * HD + 32 * md + 8 * q + 4 * hh) =
+              f32x4{c.o[md][4 * q], c.o[md][4 * q + 1], c.o[md][4 * q + 2], c.o[md][4 * q + 3]};
+      if (hh == 0) {
+        p[a.part_rows * HD + at] = c.m_run;
+        p[a.part_rows * HD + a.part_rows + at] = l;
+      }
+    }
+    return;
+  }
+  // The wave's rows leave through 4 KB of LDS, 64 channels at a time, as whole 128-byte segments: chunk c of
+  // row r at position c ^ (r % 8).
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  T* stage = reinterpret_cast<T*>(share);
+  T* obase = static_cast<T*>(a.o) + blk.b * a.o_sb + blk.h0 * a.o_sh;
+#pragma unroll
+  for (int half = 0; half < HD / 64; ++half) {
+#pragma unroll
+    for (int mm = 0; mm < 2; ++mm)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        X4 w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = (T)(c.o[2 * half + mm][4 * q + e] * inv);
+        *reinterpret_cast<X4*>(stage + n32 * 64 + (((4 * mm + q) ^ (n32 & 7)) << 3) + 4 * hh) = w;
+      }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int row = 8 * j + (lane >> 3), ch = lane & 7;
+      const X8 v = *reinterpret_cast<const X8*>(stage + row * 64 + ((ch ^ (row & 7)) << 3));
+      if (row < held) {
+        const int rr = row0 + wave * 32 + row, qi = rr / a.pack;
+        __builtin_nontemporal_store(v, reinterpret_cast<X8*>(obase + (int64_t)qi * a.o_st + (rr - qi * a.pack) * a.o_sh +
+                                                              64 * half + 8 * ch));
+      }
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   }
 }
 
@@ -564,9 +937,9 @@ __global__ __launch_bounds__(256) void masked_merge_kernel(const MaskedArgs a, i
       v[e] = fmaf(f, p0[s * a.part_floats + row * HD + (HD / 64) * lane + e], v[e]);
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  const int per = a.Hq / a.pack, b = (int)(unit / per), h0 = (int)(unit - (int64_t)b * per) * a.pack;
+  const MaskedUnit u(a, (int)unit);
   const int qi = r / a.pack;
-  T* o = static_cast<T*>(a.o) + b * a.o_sb + (int64_t)qi * a.o_st + (h0 + r - qi * a.pack) * a.o_sh + (HD / 64) * lane;
+  T* o = static_cast<T*>(a.o) + u.b * a.o_sb + (int64_t)qi * a.o_st + (u.h0 + r - qi * a.pack) * a.o_sh + (HD / 64) * lane;
 #pragma unroll
   for (int e = 0; e < HD / 64; ++e) o[e] = (T)(v[e] * inv);
 }
@@ -577,8 +950,11 @@ __global__ __launch_bounds__(256) void masked_merge_kernel(const MaskedArgs a, i
 
 template <typename T, int HD, bool CAP, bool BIAS>
 int launch_masked(MaskedArgs a, const MaskedPlan& p, hipStream_t s) {
-  hipLaunchKernelGGL((masked_step_kernel<T, HD, CAP, BIAS>), dim3((unsigned)(p.blocks * p.splits)), dim3(kStepWaves * 64),
-                     0, s, a);
+  const dim3 grid((unsigned)(p.blocks * p.splits));
+  if (p.block_rows == 32)
+    hipLaunchKernelGGL((masked_step_kernel<T, HD, CAP, BIAS>), grid, dim3(kStepWaves * 64), 0, s, a);
+  else
+    hipLaunchKernelGGL((masked_block_kernel<T, HD, CAP, BIAS>), grid, dim3(kBlockWaves * 64), 0, s, a);
   if (p.splits > 1)
     hipLaunchKernelGGL((masked_merge_kernel<T, HD>), dim3((unsigned)((p.out_rows + 3) / 4)), dim3(256), 0, s, a,
                        p.block_rows);

@@ -62,8 +62,9 @@ inline SplitPlan split_plan(int B, int H, int Lq, int keys, int cus, size_t scra
 constexpr int kMaxPosition = (1 << 30) - 1;
 // Caps above this take the form of the tanh that is exact for small arguments too.
 constexpr float kExactCap = 256.f;
-// Query heads that are rows beside each other, at most (a tile has 32 rows).
-constexpr int kMaxPack = 32;
+// Query heads that are rows beside each other, at most: as many as a wave's share of the bias entries (1016)
+// holds the distances of 32 keys and 3 positions for.
+constexpr int kMaxPack = 28;
 
 // How a call is run: `pack` query heads of one k/v head are rows of a block, `blocks` blocks of block_rows
 // rows, each as `splits` workgroups over a part of its keys.  A part's result: part_rows rows of D fp32,
@@ -78,15 +79,15 @@ inline MaskedPlan masked_plan(int B, int Hq, int Hk, int Lq, int Lk, int D, int 
   const int group = Hq / Hk;
   p.pack = group < kMaxPack ? group : kMaxPack;
   while (group % p.pack != 0) --p.pack;
-  p.block_rows = 32;
   const int64_t rows = (int64_t)Lq * p.pack;
+  p.block_rows = rows <= 32 ? 32 : kAttnWaves * 32;
   p.blocks = (rows + p.block_rows - 1) / p.block_rows * (Hq / p.pack) * B;
   p.out_rows = rows * (Hq / p.pack) * B;
   p.part_rows = (int)(rows < p.block_rows ? rows : p.block_rows);
   p.part_floats = (p.part_rows * (D + 2) + 3) / 4 * 4;
-  const int tiles = (Lk + 31) / 32;
-  int64_t n = 2 * (int64_t)cus / p.blocks;
-  if (n > (tiles + 7) / 8) n = (tiles + 7) / 8;
+  const int tiles = (Lk + kTileKeys - 1) / kTileKeys;
+  int64_t n = (p.block_rows == 32 ? 2 : 1) * (int64_t)cus / p.blocks;
+  if (n > (tiles + 3) / 4) n = (tiles + 3) / 4;
   const size_t part = (size_t)p.blocks * p.part_floats * sizeof(float);
   if (n > 1 && part * (size_t)n > scratch) n = (int64_t)(scratch / part);
   p.splits = n > 1 ? (int)n : 1;
