@@ -83,6 +83,19 @@ int launch_flash_fwd(const FlashArgs& a, hipStream_t s);
 size_t flash_split_bytes(int B, int H, int Lq, int Lk);
 
 // Attention under masks (masked_attn.h).
+// n / d for 0 <= n < 2^31 by a product and a shift: exact, since 2^(31 + s) <= m d < 2^(31 + s) + 2^s with
+// 2^s >= d.
+struct FastDiv {
+  uint32_t m;
+  int s;
+  FastDiv() = default;
+  explicit FastDiv(uint32_t d) : s(0) {
+    while ((uint64_t(1) << s) < d) ++s;
+    m = (uint32_t)(((uint64_t(1) << (31 + s)) + d - 1) / d);
+  }
+  __host__ __device__ __forceinline__ int operator()(int n) const { return (int)((uint64_t(uint32_t(n)) * m) >> (31 + s)); }
+};
+
 struct AnyTensor4 {
   const void* ptr;
   int64_t sb, st, sh;
@@ -103,11 +116,13 @@ struct MaskedArgs {
   const int32_t* q_start;    // [B] position of query row 0 (null: Lk - Lq)
   float* part;               // scratch of the key split (null: none)
   size_t part_bytes;
-  // set by the launcher (MaskedPlan)
-  int pack, splits, part_rows, part_floats;
+  // set by the launcher (MaskedPlan): blocks of rows of a unit, units times parts, and the divisions by these
+  int pack, splits, part_rows, part_floats, blocks, ups;
+  FastDiv by_pack, by_splits, by_blocks, by_batch, by_group, by_rows, by_last_ups;
 };
+constexpr int kUnitGroup = 32;    // units of a group in the order of the workgroups
 int launch_masked_attn(MaskedArgs a, int D, int dtype, hipStream_t s);
-size_t masked_split_bytes(int B, int Hq, int Hk, int Lq, int Lk, int D);
+size_t masked_split_bytes(int B, int Hq, int Hk, int Lq, int Lk, int D, bool causal);
 // CU count of the current device (cached per device after the first query).
 int device_cu_count();
 

@@ -90,13 +90,17 @@ struct MaskedCopy {
       off[u] = (uint32_t)(row * row_bytes) + col_of(row, lane);
     }
   }
+  // Tile t, all of whose keys there are, into `dst`.
+  __device__ __forceinline__ void issue_full(int t, bf16* dst, int wave) const {
+    const char* tb = base + (int64_t)(t * KEYS) * row_bytes;
+#pragma unroll
+    for (int u = 0; u < kPer; ++u) dma16_saddr(tb, off[u], lds_addr(dst + (wave + NW * u) * 512));
+  }
   // Tile t into `dst`; rows past the tensor's last key repeat it.
   __device__ __forceinline__ void issue(int t, int keys, bf16* dst, int wave, int lane) const {
     const int k0 = t * KEYS;
     if (k0 + KEYS <= keys) {
-      const char* tb = base + (int64_t)k0 * row_bytes;
-#pragma unroll
-      for (int u = 0; u < kPer; ++u) dma16_saddr(tb, off[u], lds_addr(dst + (wave + NW * u) * 512));
+      issue_full(t, dst, wave);
     } else {
 #pragma unroll
       for (int u = 0; u < kPer; ++u) {
@@ -156,16 +160,25 @@ __device__ __forceinline__ MaskedRow masked_row(const MaskedArgs& a, int b, int 
   return r;
 }
 
-// min / max over the wave's 32 rows (lanes 32 apart hold the same)
+// min / max over the wave's 32 rows (lanes 32 apart hold the same): within 16 lanes by rotations, then the two
+// halves as scalars.
+template <int N>
+__device__ __forceinline__ int row_turn(int v) {       // the value N lanes on, in the lane's 16
+  return __builtin_amdgcn_update_dpp(v, v, 0x120 + N, 0xf, 0xf, false);
+}
 __device__ __forceinline__ int rows_min(int v) {
-#pragma unroll
-  for (int m = 16; m >= 1; m >>= 1) v = min(v, __shfl_xor(v, m));
-  return __builtin_amdgcn_readfirstlane(v);
+  v = min(v, row_turn<8>(v));
+  v = min(v, row_turn<4>(v));
+  v = min(v, row_turn<2>(v));
+  v = min(v, row_turn<1>(v));
+  return min(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16));
 }
 __device__ __forceinline__ int rows_max(int v) {
-#pragma unroll
-  for (int m = 16; m >= 1; m >>= 1) v = max(v, __shfl_xor(v, m));
-  return __builtin_amdgcn_readfirstlane(v);
+  v = max(v, row_turn<8>(v));
+  v = max(v, row_turn<4>(v));
+  v = max(v, row_turn<2>(v));
+  v = max(v, row_turn<1>(v));
+  return max(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16));
 }
 
 // The sample and heads of a unit.  The samples vary fastest: units that run together are then long and
@@ -173,13 +186,12 @@ __device__ __forceinline__ int rows_max(int v) {
 struct MaskedUnit {
   int b, h0, hk;          // sample, first of the P query heads, their k/v head
   __device__ __forceinline__ MaskedUnit(const MaskedArgs& a, int unit) {
-    const int group = unit / a.B, first = group * a.pack;
+    const int group = a.by_batch(unit);
     b = uniform(unit - group * a.B);
-    h0 = uniform(first);
-    hk = uniform(first / (a.Hq / a.Hk));
+    h0 = uniform(group * a.pack);
+    hk = uniform(a.by_group(h0));
   }
-  // (divisions are vector arithmetic: their results go back to scalar registers, from which the tile
-  // copies take their addresses)
+  // (the tile copies take their addresses from scalar registers)
   static __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 };
 
@@ -187,6 +199,11 @@ struct MaskedUnit {
 struct TileRange {
   int first, end;
   __device__ __forceinline__ TileRange(int t0, int n, int part, int parts) {
+    if (parts == 1) {
+      first = t0;
+      end = t0 + n;
+      return;
+    }
     const int each = n / parts, over = n - each * parts;
     first = MaskedUnit::uniform(t0 + each * part + min(part, over));
     end = MaskedUnit::uniform(t0 + each * (part + 1) + min(part + 1, over));
@@ -202,7 +219,7 @@ struct TileRange {
 template <bool CAP, bool BIAS>
 struct ScoreMap {
   float sl2;            // scale * log2(e)
-  float cap2, k;        // cap * log2(e); 2 log2(e) scale / cap, or scale / cap with small_ok
+  float cap2, k;        // cap * log2(e); 2 log2(e) scale / cap, if precise scale / cap
   bool precise;
 
   __device__ __forceinline__ void init(const MaskedArgs& a) {
@@ -211,27 +228,27 @@ struct ScoreMap {
     precise = a.cap > kExactCap;
     k = CAP ? (precise ? a.scale / a.cap : 2.f * kLog2e * a.scale / a.cap) : 0.f;
   }
-  // Scores in units of log2(e), without bias.
+  // Scores in units of log2(e), without bias (without cap and bias: as they are).
   // tanh(y) = 1 - 2 / (1 + e^2y): off by 2^-22 of the cap at most, which up to caps of 256 is less than the
-  // rounding of the softmax weights; beyond, small y go by the series y - y^3/3 + 2 y^5/15.
+  // rounding of the softmax weights; beyond (`precise`), small y go by the series y - y^3/3 + 2 y^5/15.
+  __device__ __forceinline__ float one(float s) const {
+    if constexpr (CAP) return fmaf(-2.f * cap2, __builtin_amdgcn_rcpf(1.f + fast_exp2(s * k)), cap2);
+    else if constexpr (BIAS) return s * sl2;
+    else return s;
+  }
+  template <bool SMALL = false>       // SMALL: the cap is known not to be `precise`
   __device__ __forceinline__ void map(f32x16& s) const {
-    if constexpr (CAP) {
-      if (precise) {
+    if (CAP && !SMALL && precise) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const float y = s[r] * k, y2 = y * y;
-          const float far = fmaf(-2.f, __builtin_amdgcn_rcpf(1.f + fast_exp2(y * (2.f * kLog2e))), 1.f);
-          const float near = fmaf(y * y2, fmaf(y2, 2.f / 15.f, -1.f / 3.f), y);
-          s[r] = cap2 * (fabsf(y) < 0.1f ? near : far);
-        }
-      } else {
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          s[r] = fmaf(-2.f * cap2, __builtin_amdgcn_rcpf(1.f + fast_exp2(s[r] * k)), cap2);
+      for (int r = 0; r < 16; ++r) {
+        const float y = s[r] * k, y2 = y * y;
+        const float far = fmaf(-2.f, __builtin_amdgcn_rcpf(1.f + fast_exp2(y * (2.f * kLog2e))), 1.f);
+        const float near = fmaf(y * y2, fmaf(y2, 2.f / 15.f, -1.f / 3.f), y);
+        s[r] = cap2 * (fabsf(y) < 0.1f ? near : far);
       }
-    } else if constexpr (BIAS) {
+    } else {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] *= sl2;
+      for (int r = 0; r < 16; ++r) s[r] = one(s[r]);
     }
   }
   // exponent of a score against the reference point m
@@ -395,7 +412,7 @@ struct WaveRows {
   // rows row0 .. row0 + 31 of a unit; those past the last one repeat it (they are not stored)
   __device__ __forceinline__ WaveRows(const MaskedArgs& a, int b, int row0, int rows, int lane) {
     const int r = min(row0 + (lane & 31), rows - 1);
-    i = r / a.pack;
+    i = a.by_pack(r);
     g = r - i * a.pack;
     m = masked_row(a, b, i);
     const bool some = m.lo < m.hi;
@@ -444,6 +461,7 @@ __device__ __forceinline__ void attend_wave(const MaskedArgs& a, const MaskedUni
   m_run = -FLT_MAX;
   l_run = 0.f;
 
+  wait_vm_all();      // (as in the block kernel: the query rows are there for the compiler too)
   for (int slot = 0; t < tb; t += stride, slot = SLOTS == 1 ? 0 : slot ^ 1) {
     const int kt = t * kWaveKeys;
     const bf16 *Kt = tiles + slot * (2 * kTile), *Vt = Kt + kTile;
@@ -518,10 +536,10 @@ __global__ __launch_bounds__(kStepWaves * 64, 1) void masked_step_kernel(const M
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n32 = lane & 31, hh = lane >> 5;
-  const int rows = a.Lq * a.pack, blocks = (rows + 31) / 32;
-  const int block = blockIdx.x / a.splits, part = blockIdx.x - block * a.splits;
-  const MaskedUnit blk(a, block / blocks);
-  const int row0 = block % blocks * 32;
+  const int rows = a.Lq * a.pack;
+  const int block = a.by_splits(blockIdx.x), part = blockIdx.x - block * a.splits;
+  const int unit = a.by_blocks(block), row0 = (block - unit * a.blocks) * 32;
+  const MaskedUnit blk(a, unit);
   const WaveRows w(a, blk.b, row0, rows, lane);
   const int t0 = w.first / kWaveKeys;
   const TileRange range(t0, w.first < w.end ? (w.end - 1) / kWaveKeys + 1 - t0 : 0, part, a.splits);
@@ -575,7 +593,7 @@ __global__ __launch_bounds__(kStepWaves * 64, 1) void masked_step_kernel(const M
       }
     } else {
       const float inv = l == 0.f ? 0.f : 1.f / l;
-      const int rr = row0 + row, qi = rr / a.pack;
+      const int rr = row0 + row, qi = a.by_pack(rr);
       X8 y;
 #pragma unroll
       for (int e = 0; e < 8; ++e) y[e] = (T)(v[e] * inv);
@@ -586,11 +604,32 @@ __global__ __launch_bounds__(kStepWaves * 64, 1) void masked_step_kernel(const M
 }
 
 // ---------------------------------------------------------------------------
-// many rows: 256 rows a workgroup, 32 a wave, on tiles of 64 keys that all waves share
+// many rows: 32 a wave, on tiles of 64 keys that a workgroup's waves share
 // ---------------------------------------------------------------------------
+//
+// KG = 1: eight waves of rows (256).  KG = 2: four (128), the other four waves are the same rows on every
+// second tile; a block then takes half as many steps, which is what a launch with few, or unequally long,
+// blocks ends sooner by, for twice the tile copies.
 
 constexpr int kBlockWaves = kAttnWaves, kBlockKeys = kTileKeys;
 constexpr int kBlockWindow = 8128;      // bias entries of a workgroup
+
+// The order of the workgroups: units (and their parts) in groups of kUnitGroup, in a group the last rows of all
+// its units first.  Under a causal mask those see the most keys, so that the short blocks fill the end of the
+// launch.  Workgroup i runs on XCD i % 8: the blocks of a unit share one L2 where the units of a group are a
+// multiple of 8, and where they are fewer each unit's long and short blocks spread evenly over the XCDs.
+struct BlockOrder {
+  int up, rb;
+  __device__ __forceinline__ BlockOrder(const MaskedArgs& a, int id) {
+    const int group = a.by_blocks(id / kUnitGroup), in = id - group * (kUnitGroup * a.blocks);
+    // (the last group may be smaller)
+    const bool whole = (group + 1) * kUnitGroup <= a.ups;
+    const int size = whole ? kUnitGroup : a.ups - group * kUnitGroup;
+    const int at = whole ? in / kUnitGroup : a.by_last_ups(in);
+    up = group * kUnitGroup + (in - at * size);
+    rb = a.blocks - 1 - at;
+  }
+};
 
 // The arithmetic of a wave's 32 rows on a tile of 64 keys (scores c0: keys 0 .. 31, c1: 32 .. 63).
 template <typename T, int HD, bool CAP, bool BIAS>
@@ -624,8 +663,8 @@ struct BlockCore {
     }
   }
 
-  __device__ __forceinline__ void weigh(const f32x16& c, int r, X8 pb[2], float& acc) const {
-    const X2 w = {(T)map.weight(c[r], m_run), (T)map.weight(c[r + 1], m_run)};
+  __device__ __forceinline__ void weigh(const f32x16& c, int r, float m, X8 pb[2], float& acc) const {
+    const X2 w = {(T)map.weight(c[r], m), (T)map.weight(c[r + 1], m)};
     pb[r >> 3][r & 7] = w[0];
     pb[r >> 3][(r & 7) + 1] = w[1];
     acc = Elem<T>::add2(w, acc);
@@ -634,12 +673,15 @@ struct BlockCore {
   // The weights of a tile and this lane's sum of them (of the rounded values that the products use), eight
   // exponentials in flight at most.
   __device__ __forceinline__ float exp_tile(const f32x16& c0, const f32x16& c1, X8 pb[4]) const {
-    float acc[2] = {0.f, 0.f};
+    float acc[2] = {0.f, 0.f}, m = m_run;
+    // (a value of its own for the compiler, which otherwise moves this and qk_exp's exponents out of the branch
+    // between them, in front of the MFMAs that they are to run beside)
+    asm volatile("" : "+v"(m));
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int r = 0; r < 16; r += 2) {
-        weigh(h == 0 ? c0 : c1, r, pb + 2 * h, acc[h]);
+        weigh(h == 0 ? c0 : c1, r, m, pb + 2 * h, acc[h]);
         if ((r & 7) == 6) __builtin_amdgcn_sched_barrier(0);
       }
     return acc[0] + acc[1];
@@ -661,8 +703,8 @@ struct BlockCore {
       n1 = Elem<T>::mfma(a1, op.qf[ks], ks == 0 ? f32x16{} : n1);
 #pragma unroll
       for (int r = kEach * ks; r < kEach * (ks + 1); r += 2) {
-        weigh(c0, r, pb, acc0);
-        weigh(c1, r, pb + 2, acc1);
+        weigh(c0, r, m_run, pb, acc0);
+        weigh(c1, r, m_run, pb + 2, acc1);
       }
       if (ks < kSteps - 1) {
         a0 = b0;
@@ -708,13 +750,14 @@ struct BlockCore {
   }
 };
 
-template <typename T, int HD, bool CAP, bool BIAS>
+template <typename T, int HD, bool CAP, bool BIAS, int KG>
 __global__ __launch_bounds__(kBlockWaves * 64, 2) void masked_block_kernel(const MaskedArgs a) {
   typedef typename Elem<T>::x8 X8;
   typedef typename Elem<T>::x4 X4;
-  constexpr int BM = kBlockWaves * 32, BK = kBlockKeys, kTile = BK * HD;
-  // Rings of four k and v tiles and a barrier every second tile, as in the unmasked kernel: an even step
-  // issues the copies of the next pair of tiles, the odd one waits for them.
+  constexpr int kRowWaves = kBlockWaves / KG, BM = kRowWaves * 32, BK = kBlockKeys, kTile = BK * HD;
+  // Rings of four k and v tiles and a barrier every second tile.  With KG = 1, as in the unmasked kernel, an
+  // even step issues the copies of the next pair of tiles and the odd one waits for them; with KG = 2 a step
+  // is a pair of tiles.
   __shared__ __attribute__((aligned(1024))) bf16 k_lds[4][kTile];
   __shared__ __attribute__((aligned(1024))) bf16 v_lds[4][kTile];
   __shared__ float window[BIAS ? kBlockWindow : 1];
@@ -723,19 +766,31 @@ __global__ __launch_bounds__(kBlockWaves * 64, 2) void masked_block_kernel(const
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n32 = lane & 31, hh = lane >> 5;
-  const int rows = a.Lq * a.pack, blocks = (rows + BM - 1) / BM;
-  // Each XCD runs contiguous numbers: the blocks of one unit and part share k and v in its L2.  The last rows
-  // come first, under a causal mask they see the most keys.
-  const int id = xcd_remap(blockIdx.x, gridDim.x);
-  const int up = id / blocks, unit = up / a.splits, part = up - unit * a.splits;
-  const int row0 = MaskedUnit::uniform((blocks - 1 - (id - up * blocks)) * BM);
+  const int rows = a.Lq * a.pack;
+  const BlockOrder order(a, blockIdx.x);
+  const int unit = a.by_splits(order.up), part = order.up - unit * a.splits;
+  const int row0 = MaskedUnit::uniform(order.rb * BM);
   const MaskedUnit blk(a, unit);
-  const bool live = row0 + wave * 32 < rows;      // (a wave without rows copies its share and meets the barriers)
-  WaveRows w(a, blk.b, row0 + wave * 32, rows, lane);
+  const int kg = wave / kRowWaves, wrow0 = row0 + (wave - kg * kRowWaves) * 32;
+  const bool live = wrow0 < rows;      // (a wave without rows copies its share and meets the barriers)
+  WaveRows w(a, blk.b, wrow0, rows, lane);
   if (!live) {
     w.first = 0x7fffffff;
     w.end = 0;
   }
+  // What the first tile needs goes out before it is known which tiles these rows see: without documents, and
+  // not split, they begin with tile 0 (if they see any).
+  MaskedCopy<HD, BK, kBlockWaves, false> kc;
+  MaskedCopy<HD, BK, kBlockWaves, true> vc;
+  kc.init(static_cast<const T*>(a.k.ptr) + blk.b * a.k.sb + blk.hk * a.k.sh, a.k.st, wave, lane);
+  vc.init(static_cast<const T*>(a.v.ptr) + blk.b * a.v.sb + blk.hk * a.v.sh, a.v.st, wave, lane);
+  const bool early = a.doc_starts == nullptr && a.splits == 1 && a.Lk > 0;
+  if (early) {
+    kc.issue(0, a.Lk, k_lds[0], wave, lane);
+    vc.issue(0, a.Lk, v_lds[0], wave, lane);
+  }
+  BlockCore<T, HD, CAP, BIAS> c;
+  c.op.init(static_cast<const T*>(a.q.ptr) + blk.b * a.q.sb + (int64_t)w.i * a.q.st + (blk.h0 + w.g) * a.q.sh, lane);
   // the tiles that any row of the workgroup sees keys of, this part of them
   if (lane == 0) {
     ends[0][wave] = w.first;
@@ -751,35 +806,32 @@ __global__ __launch_bounds__(kBlockWaves * 64, 2) void masked_block_kernel(const
   const TileRange range(first / BK, first < end ? (end - 1) / BK + 1 - first / BK : 0, part, a.splits);
   const int nt = range.end - range.first;
 
-  BlockCore<T, HD, CAP, BIAS> c;
   bool bad = false;       // a tile that needed a mask held a NaN or an infinity in v
   c.reset();
   c.map.init(a);
   if (nt > 0) {
-    MaskedCopy<HD, BK, kBlockWaves, false> kc;
-    MaskedCopy<HD, BK, kBlockWaves, true> vc;
-    kc.init(static_cast<const T*>(a.k.ptr) + blk.b * a.k.sb + blk.hk * a.k.sh, a.k.st, wave, lane);
-    vc.init(static_cast<const T*>(a.v.ptr) + blk.b * a.v.sb + blk.hk * a.v.sh, a.v.st, wave, lane);
     auto copy_k = [&](int u) {
       if (u < nt) kc.issue(range.first + u, a.Lk, k_lds[u & 3], wave, lane);
     };
     auto copy_v = [&](int u) {
       if (u < nt) vc.issue(range.first + u, a.Lk, v_lds[u & 3], wave, lane);
     };
-    copy_k(0);
-    copy_v(0);
+    if (!early) {
+      copy_k(0);
+      copy_v(0);
+    }
     copy_k(1);
     copy_v(1);
     copy_k(2);
-    c.op.init(static_cast<const T*>(a.q.ptr) + blk.b * a.q.sb + (int64_t)w.i * a.q.st + (blk.h0 + w.g) * a.q.sh, lane);
+    if (KG == 2) copy_k(3);
 
     BiasWindow win;
     int p_first = 0, p_last = 0;       // positions of the workgroup's rows
     if constexpr (BIAS) {
       win.init(kBlockWindow, a.pack);
       const int at = MaskedUnit::uniform(w.m.p - w.i);
-      p_first = at + row0 / a.pack;
-      p_last = at + (min(row0 + BM, rows) - 1) / a.pack;
+      p_first = at + a.by_pack(row0);
+      p_last = at + a.by_pack(min(row0 + BM, rows) - 1);
     }
     // whether the wave's rows see any key of tile u
     auto seen = [&](int u) {
@@ -787,36 +839,42 @@ __global__ __launch_bounds__(kBlockWaves * 64, 2) void masked_block_kernel(const
       return u < nt && kt < w.end && kt + BK > w.first;
     };
     bool fresh = true;
-    auto step = [&](int u, f32x16& c0, f32x16& c1, f32x16& n0, f32x16& n1) {
-      const int kt = (range.first + u) * BK;
-      if constexpr (BIAS) {
-        if (!win.holds(kt - p_last, kt + BK - 1 - p_first)) {
+    const int base = range.first * BK, last = range.end - 1;
+    // One step: tiles u0 (.. u0 + KG - 1), this wave's its u.  LEAN: every row sees all of tile u, some see
+    // tile u + KG, and the tiles to be copied are whole, so that no such question is asked (past the last one
+    // it is copied again).
+    auto step = [&](auto lean, int u0, f32x16& c0, f32x16& c1, f32x16& n0, f32x16& n1) {
+      constexpr bool LEAN = decltype(lean)::value;
+      const int u = u0 + kg, kt = (range.first + u) * BK;
+      if constexpr (BIAS && !LEAN) {
+        const int k0 = (range.first + u0) * BK;
+        if (!win.holds(k0 - p_last, k0 + KG * BK - 1 - p_first)) {
           __syncthreads();
-          win.load(a, blk.h0, kt - p_last, (int64_t)(nt - u) * BK + (p_last - p_first), window, threadIdx.x,
+          win.load(a, blk.h0, k0 - p_last, (int64_t)(nt - u0 + KG - 1) * BK + (p_last - p_first), window, threadIdx.x,
                    kBlockWaves * 64);
           __syncthreads();
         }
       }
-      const bool here = seen(u), next = seen(u + 1);
-      const bool masked = here && (kt < w.all_lo || kt + BK > w.all_hi);
-      const bf16 *Kn = k_lds[(u + 1) & 3], *Vt = v_lds[u & 3];
+      const bool here = LEAN || seen(u), next = LEAN || seen(u + KG);
+      const bool masked = !LEAN && here && (kt < w.all_lo || kt + BK > w.all_hi);
+      const bf16 *Kn = k_lds[(u + KG) & 3], *Vt = v_lds[u & 3];
       X8 pb[4];
       if (here) {
-        c.map.map(c0);
-        c.map.map(c1);
+        c.map.template map<LEAN>(c0);
+        c.map.template map<LEAN>(c1);
         if constexpr (BIAS) {
-          const float* e0 = window + w.g * win.per + (kt + 4 * hh - w.m.p - win.w0);
+          const float* bias = window + w.g * win.per + (kt + 4 * hh - w.m.p - win.w0);
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            c0[e] += e0[8 * (e >> 2) + (e & 3)];
-            c1[e] += e0[32 + 8 * (e >> 2) + (e & 3)];
+            c0[e] += bias[8 * (e >> 2) + (e & 3)];
+            c1[e] += bias[32 + 8 * (e >> 2) + (e & 3)];
           }
         }
         if (masked) {
           mask_scores(c0, kt, hh, w.m);
           mask_scores(c1, kt + 32, hh, w.m);
         }
-        if (fresh) {
+        if (!LEAN && fresh) {
           c.m_run = fmaxf(-FLT_MAX, c.tile_top(c0, c1));
           fresh = false;
         }
@@ -825,47 +883,110 @@ __global__ __launch_bounds__(kBlockWaves * 64, 2) void masked_block_kernel(const
       } else if (next) {
         c.qk(Kn, n0, n1);
       }
-      if ((u & 1) == 0) {
-        copy_k(u + 3);
-        copy_k(u + 4);
-        copy_v(u + 2);
-        copy_v(u + 3);
+      if (KG == 2 || (u0 & 1) == 0) {
+        if constexpr (LEAN) {
+          kc.issue_full(min(range.first + u0 + 2 + KG, last), k_lds[(u0 + 2 + KG) & 3], wave);
+          kc.issue_full(min(range.first + u0 + 3 + KG, last), k_lds[(u0 + 3 + KG) & 3], wave);
+          vc.issue_full(min(range.first + u0 + 2, last), v_lds[(u0 + 2) & 3], wave);
+          vc.issue_full(min(range.first + u0 + 3, last), v_lds[(u0 + 3) & 3], wave);
+        } else {
+          copy_k(u0 + 2 + KG);
+          copy_k(u0 + 3 + KG);
+          copy_v(u0 + 2);
+          copy_v(u0 + 3);
+        }
       }
       if (here) {
         if (masked) bad = bad || tile_not_finite<T, HD, BK>(Vt, lane);
         c.pv(pb, Vt);
       }
-      if (u & 1) {
+      if (KG == 2 || (u0 & 1)) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
       }
     };
+    // Two steps from u0 on are lean for this wave if lean_lo <= u0 < lean_hi (and it has begun).
+    const int seen_end = min(nt, (w.end - 1 - base) / BK + 1);
+    const int lean_lo = (w.all_lo - base + BK - 1) / BK - kg;
+    const int lean_hi = min(min((w.all_hi - base) / BK - KG, seen_end - 2 * KG) - kg,
+                            range.end * BK <= a.Lk ? nt : nt - 1 - (KG == 1 ? 4 : 7));
 
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    // (the compiler's own wait: it must know here that the query rows are there, or it waits for them, and so for
+    // every copy in flight, at their first use in each step)
+    wait_vm_all();
     __syncthreads();
     f32x16 sa0, sa1, sb0, sb1;
-    if (seen(0)) c.qk(k_lds[0], sa0, sa1);
-    __syncthreads();      // every wave is done with tile 0 of k before it is overwritten
-    for (int u = 0; u < nt; u += 2) {
-      step(u, sa0, sa1, sb0, sb1);
-      if (u + 1 < nt) step(u + 1, sb0, sb1, sa0, sa1);
+    if (seen(kg)) {
+      c.qk(k_lds[kg], sa0, sa1);
+      // The first reference point, where every row sees the whole tile.  (With a bias it needs the mapped scores:
+      // one that lies above all of a row's would leave it no weights.)
+      if (!BIAS && lean_lo <= 0 && base + (kg + 1) * BK <= w.all_hi && !(CAP && c.map.precise)) {
+        c.m_run = c.map.top(c.map.one(pair_max(fmaxf(max16(sa0), max16(sa1)))));
+        fresh = !(c.m_run >= -FLT_MAX && c.m_run <= FLT_MAX);
+        if (__builtin_amdgcn_ballot_w64(fresh) != 0) c.m_run = -FLT_MAX;
+        fresh = __builtin_amdgcn_ballot_w64(fresh) != 0;
+      }
     }
+    __syncthreads();      // every wave is done with the first tiles of k before they are overwritten
+    for (int u = 0; u < nt; u += 2 * KG) {
+      while (u >= lean_lo && u < lean_hi && !fresh && !(CAP && c.map.precise) &&
+             (!BIAS || win.holds(base + u * BK - p_last, base + (u + 2 * KG) * BK - 1 - p_first))) {
+        step(std::true_type{}, u, sa0, sa1, sb0, sb1);
+        step(std::true_type{}, u + KG, sb0, sb1, sa0, sa1);
+        u += 2 * KG;
+      }
+      if (u < nt) step(std::false_type{}, u, sa0, sa1, sb0, sb1);
+      if (u + KG < nt) step(std::false_type{}, u + KG, sb0, sb1, sa0, sa1);
+    }
+    if (KG == 2 && lane == 0) ends[0][wave] = bad;
     __syncthreads();      // ... and with the last tiles before the output is staged over them
+    if (KG == 2) bad = ends[0][wave % kRowWaves] | ends[0][wave % kRowWaves + kRowWaves];
+  } else {
+    wait_vm_all();        // (tile 0 has landed before its place is used otherwise)
+    __syncthreads();
   }
-  if (!live) return;
+  if (KG == 1 && !live) return;
   // This wave's share of the rings, from here on.
   bf16* const share = wave < 4 ? k_lds[wave] : v_lds[wave - 4];
   // Such a value may have reached rows that do not see it: the wave's rows once more, by itself.  (Told apart in
   // the loop above, the second way to form O left it too few registers: 40 were spilled in every tile.)
   if (bad)
-    attend_wave<T, HD, CAP, BIAS, 1>(a, blk, w, max(range.first * (BK / kWaveKeys), w.first / kWaveKeys),
-                                     min(range.end * (BK / kWaveKeys), (w.end - 1) / kWaveKeys + 1), 1,
-                                     share, window + wave * (kBlockWindow / kBlockWaves), kBlockWindow / kBlockWaves,
-                                     lane, c.o, c.m_run, c.l_run);
+    attend_wave<T, HD, CAP, BIAS, 1>(a, blk, w, max(range.first * (BK / kWaveKeys), w.first / kWaveKeys) + kg,
+                                     min(range.end * (BK / kWaveKeys), (w.end - 1) / kWaveKeys + 1), KG, share,
+                                     window + wave * (kBlockWindow / kBlockWaves), kBlockWindow / kBlockWaves, lane, c.o,
+                                     c.m_run, c.l_run);
+  if constexpr (KG == 2) {
+    // The second four waves leave what they have to the first: the rows lie in the same lanes.
+    float* const other = reinterpret_cast<float*>(&v_lds[0][0]) + (wave % kRowWaves) * (kTile / 2) + lane * 4;
+    float* const stat = reinterpret_cast<float*>(&k_lds[0][0]) + (wave % kRowWaves) * (kTile / 2) + lane;
+    __syncthreads();      // (the share of a wave that went over its rows again is read no more)
+    if (kg == 1) {
+#pragma unroll
+      for (int n = 0; n < HD / 8; ++n)
+        *reinterpret_cast<f32x4*>(other + n * 256) = f32x4{c.o[n / 4][4 * (n & 3)], c.o[n / 4][4 * (n & 3) + 1],
+                                                           c.o[n / 4][4 * (n & 3) + 2], c.o[n / 4][4 * (n & 3) + 3]};
+      stat[0] = c.m_run;
+      stat[64] = c.l_run;
+    }
+    __syncthreads();
+    if (kg == 1 || !live) return;
+    const float m1 = stat[0], top = fmaxf(c.m_run, m1);
+    const float f0 = fast_exp2(c.m_run - top), f1 = fast_exp2(m1 - top);
+    c.m_run = top;
+    c.l_run = f0 * c.l_run + f1 * stat[64];
+#pragma unroll
+    for (int n = 0; n < HD / 8; ++n) {
+      const f32x4 v = *reinterpret_cast<const f32x4*>(other + n * 256);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) c.o[n / 4][4 * (n & 3) + e] = f0 * c.o[n / 4][4 * (n & 3) + e] + f1 * v[e];
+    }
+    // (all of it read before the rows are staged over it)
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  }
   const float l = pair_sum(c.l_run);
-  const int held = min(rows - row0 - wave * 32, 32);        // rows of this wave
+  const int held = min(rows - wrow0, 32);        // rows of this wave
   if (a.splits > 1) {
-    const int block = unit * blocks + row0 / BM, at = wave * 32 + n32;
+    const int block = unit * a.blocks + row0 / BM, at = wrow0 - row0 + n32;
     float* p = a.part + ((int64_t)block * a.splits + part) * a.part_floats;
     if (n32 < held) {
 #pragma unroll
@@ -903,7 +1024,7 @@ __global__ __launch_bounds__(kBlockWaves * 64, 2) void masked_block_kernel(const
       const int row = 8 * j + (lane >> 3), ch = lane & 7;
       const X8 v = *reinterpret_cast<const X8*>(stage + row * 64 + ((ch ^ (row & 7)) << 3));
       if (row < held) {
-        const int rr = row0 + wave * 32 + row, qi = rr / a.pack;
+        const int rr = wrow0 + row, qi = a.by_pack(rr);
         __builtin_nontemporal_store(v, reinterpret_cast<X8*>(obase + (int64_t)qi * a.o_st + (rr - qi * a.pack) * a.o_sh +
                                                               64 * half + 8 * ch));
       }
@@ -912,36 +1033,39 @@ __global__ __launch_bounds__(kBlockWaves * 64, 2) void masked_block_kernel(const
   }
 }
 
-// Rows whose keys were split: O = sum_i w_i O_i / sum_i w_i l_i with w_i = exp2(m_i - max m).  A wave a row.
+// Rows whose keys were split: O = sum_i w_i O_i / sum_i w_i l_i with w_i = exp2(m_i - max m).  A row has HD / 4
+// lanes, four channels each.
 template <typename T, int HD>
-__global__ __launch_bounds__(256) void masked_merge_kernel(const MaskedArgs a, int block_rows) {
-  const int lane = threadIdx.x & 63;
-  const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int rows = a.Lq * a.pack, blocks = (rows + block_rows - 1) / block_rows;
-  const int64_t unit = id / rows;
-  if (unit >= (int64_t)a.B * (a.Hq / a.pack)) return;
-  const int r = (int)(id - unit * rows), rb = r / block_rows, row = r - rb * block_rows;
-  const float* p0 = a.part + (unit * blocks + rb) * a.splits * a.part_floats;
+__global__ __launch_bounds__(256) void masked_merge_kernel(const MaskedArgs a, int out_rows, int block_shift) {
+  typedef typename Elem<T>::x4 X4;
+  constexpr int kLanes = HD / 4;
+  const int lane = threadIdx.x % kLanes, id = blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
+  if (id >= out_rows) return;
+  const int unit = a.by_rows(id);
+  const int r = id - unit * (a.Lq * a.pack), rb = r >> block_shift, row = r - (rb << block_shift);
+  const float* p0 = a.part + ((int64_t)unit * a.blocks + rb) * a.splits * a.part_floats;
   const float* st = p0 + a.part_rows * HD + row;
   float top = -FLT_MAX;
-  for (int s = lane; s < a.splits; s += 64) top = fmaxf(top, st[s * a.part_floats]);
+  for (int s = lane; s < a.splits; s += kLanes) top = fmaxf(top, st[(int64_t)s * a.part_floats]);
 #pragma unroll
-  for (int x = 32; x >= 1; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
-  float v[HD / 64] = {}, l = 0.f;
+  for (int x = kLanes / 2; x >= 1; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
+  f32x4 v = {};
+  float l = 0.f;
+#pragma unroll 4
   for (int s = 0; s < a.splits; ++s) {
-    const float* q = st + s * a.part_floats;
+    const float* q = st + (int64_t)s * a.part_floats;
+    const f32x4 o = *reinterpret_cast<const f32x4*>(p0 + (int64_t)s * a.part_floats + row * HD + 4 * lane);
     const float f = fast_exp2(q[0] - top);
     l += f * q[a.part_rows];
-#pragma unroll
-    for (int e = 0; e < HD / 64; ++e)
-      v[e] = fmaf(f, p0[s * a.part_floats + row * HD + (HD / 64) * lane + e], v[e]);
+    v += f * o;
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  const MaskedUnit u(a, (int)unit);
-  const int qi = r / a.pack;
-  T* o = static_cast<T*>(a.o) + u.b * a.o_sb + (int64_t)qi * a.o_st + (u.h0 + r - qi * a.pack) * a.o_sh + (HD / 64) * lane;
+  const int group = a.by_batch(unit), b = unit - group * a.B, qi = a.by_pack(r);
+  X4 y;
 #pragma unroll
-  for (int e = 0; e < HD / 64; ++e) o[e] = (T)(v[e] * inv);
+  for (int e = 0; e < 4; ++e) y[e] = (T)(v[e] * inv);
+  *reinterpret_cast<X4*>(static_cast<T*>(a.o) + b * a.o_sb + (int64_t)qi * a.o_st +
+                         (group * a.pack + r - qi * a.pack) * a.o_sh + 4 * lane) = y;
 }
 
 // ---------------------------------------------------------------------------
@@ -953,11 +1077,14 @@ int launch_masked(MaskedArgs a, const MaskedPlan& p, hipStream_t s) {
   const dim3 grid((unsigned)(p.blocks * p.splits));
   if (p.block_rows == 32)
     hipLaunchKernelGGL((masked_step_kernel<T, HD, CAP, BIAS>), grid, dim3(kStepWaves * 64), 0, s, a);
+  else if (p.block_rows == 128)
+    hipLaunchKernelGGL((masked_block_kernel<T, HD, CAP, BIAS, 2>), grid, dim3(kBlockWaves * 64), 0, s, a);
   else
-    hipLaunchKernelGGL((masked_block_kernel<T, HD, CAP, BIAS>), grid, dim3(kBlockWaves * 64), 0, s, a);
+    hipLaunchKernelGGL((masked_block_kernel<T, HD, CAP, BIAS, 1>), grid, dim3(kBlockWaves * 64), 0, s, a);
   if (p.splits > 1)
-    hipLaunchKernelGGL((masked_merge_kernel<T, HD>), dim3((unsigned)((p.out_rows + 3) / 4)), dim3(256), 0, s, a,
-                       p.block_rows);
+    hipLaunchKernelGGL((masked_merge_kernel<T, HD>), dim3((unsigned)((p.out_rows + 1024 / HD - 1) / (1024 / HD))),
+                       dim3(256), 0, s, a,
+                       (int)p.out_rows, p.block_rows == 32 ? 5 : p.block_rows == 128 ? 7 : 8);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? 0 : set_error(4, "masked_attn launch: %s", hipGetErrorString(e));
 }

@@ -74,24 +74,61 @@ struct MaskedPlan {
   int64_t blocks, out_rows;
   size_t bytes;
 };
-inline MaskedPlan masked_plan(int B, int Hq, int Hk, int Lq, int Lk, int D, int cus, size_t scratch) {
+// Up to this many rows of a unit go by tiles of 32 rows, whose waves split the keys, more by blocks of 256.
+constexpr int kStepRows = 32;
+constexpr int kMaskedMaxSplits = 64;
+constexpr float kBlockUs = 3.f, kMaskedMergeUs = 4.f;
+inline MaskedPlan masked_plan(int B, int Hq, int Hk, int Lq, int Lk, int D, bool causal, int cus, size_t scratch) {
   MaskedPlan p{};
   const int group = Hq / Hk;
   p.pack = group < kMaxPack ? group : kMaxPack;
   while (group % p.pack != 0) --p.pack;
-  const int64_t rows = (int64_t)Lq * p.pack;
-  p.block_rows = rows <= 32 ? 32 : kAttnWaves * 32;
-  p.blocks = (rows + p.block_rows - 1) / p.block_rows * (Hq / p.pack) * B;
-  p.out_rows = rows * (Hq / p.pack) * B;
-  p.part_rows = (int)(rows < p.block_rows ? rows : p.block_rows);
-  p.part_floats = (p.part_rows * (D + 2) + 3) / 4 * 4;
-  const int tiles = (Lk + kTileKeys - 1) / kTileKeys;
-  int64_t n = (p.block_rows == 32 ? 2 : 1) * (int64_t)cus / p.blocks;
-  if (n > (tiles + 3) / 4) n = (tiles + 3) / 4;
-  const size_t part = (size_t)p.blocks * p.part_floats * sizeof(float);
-  if (n > 1 && part * (size_t)n > scratch) n = (int64_t)(scratch / part);
-  p.splits = n > 1 ? (int)n : 1;
-  p.bytes = p.splits > 1 ? part * p.splits : 0;
+  const int64_t rows = (int64_t)Lq * p.pack, units = (int64_t)(Hq / p.pack) * B;
+  p.out_rows = rows * units;
+  const int nt = (Lk + kTileKeys - 1) / kTileKeys;
+  // blocks of `block_rows` rows, `n` parts: whether the scratch holds them
+  auto layout = [&](int block_rows, int n) {
+    p.block_rows = block_rows;
+    p.blocks = (rows + block_rows - 1) / block_rows * units;
+    p.part_rows = (int)(rows < block_rows ? rows : block_rows);
+    p.part_floats = (p.part_rows * (D + 2) + 3) / 4 * 4;
+    p.splits = n;
+    p.bytes = n > 1 ? (size_t)p.blocks * p.part_floats * sizeof(float) * n : 0;
+    return p.bytes <= scratch;
+  };
+  if (rows <= kStepRows) {
+    int64_t n = 2 * (int64_t)cus / units;
+    if (n > (nt + 3) / 4) n = (nt + 3) / 4;
+    if (n > kMaskedMaxSplits) n = kMaskedMaxSplits;
+    if (n < 1) n = 1;
+    while (!layout(32, (int)n)) --n;
+    return p;
+  }
+  // Of a block's tiles (nt at most) a workgroup, one a CU, takes `step` us each, with 128 rows for each pair, and
+  // kBlockUs besides.  Without a causal mask the blocks run in rounds; with one the longest come first and the
+  // launch ends with the longest or when the sum of all is done.  A split costs the merge launch and the
+  // parts' way through memory.
+  const float mean = causal ? nt - 0.5f * ((Lq < Lk ? Lq : Lk) / kTileKeys) : (float)nt;
+  float best = 0.f;
+  int best_rows = 0, best_n = 1;
+  for (int block_rows = 256; block_rows >= 128; block_rows /= 2) {
+    const int pair = 256 / block_rows;
+    const float step = D == 128 ? (pair == 1 ? 1.9f : 2.05f) : (pair == 1 ? 1.15f : 1.25f);
+    for (int n = 1; n <= kMaskedMaxSplits && (n == 1 || n * 4 * pair <= nt); ++n) {
+      if (!layout(block_rows, n)) break;
+      const float longest = step * ((nt + n * pair - 1) / (n * pair)) + kBlockUs;
+      const float sum = p.blocks * n * (step * (mean / (n * pair) + 0.5f) + kBlockUs) / cus;
+      const float rounds = (float)((p.blocks * n + cus - 1) / cus) * longest;
+      float us = causal ? (sum > longest ? sum : longest) : rounds;
+      if (n > 1) us += kMaskedMergeUs + p.bytes * (2.f / 1e7f);
+      if (best_rows == 0 || us < 0.95f * best) {
+        best = us;
+        best_rows = block_rows;
+        best_n = n;
+      }
+    }
+  }
+  layout(best_rows, best_n);
   return p;
 }
 
