@@ -125,7 +125,7 @@ int wan_flash_attn_qnorm_ws(wan_tensor q, wan_tensor k, wan_tensor v, wan_tensor
  * v rows of keys that a row does not see do not reach it, whatever they hold.  The arrays are on the device
  * and int32: values outside their ranges are clamped, doc_starts that do not ascend give other documents,
  * never a read out of range.  `workspace` is optional scratch of wan_masked_attn_workspace() bytes, 256-byte
- * aligned (0: not needed): with it calls whose rows leave compute units idle split their keys over them,
+ * aligned (for this mask; 0: not needed): with it calls whose rows leave compute units idle split their keys over them,
  * with fewer bytes less far.
  */
 typedef struct wan_attn_mask {
@@ -142,7 +142,7 @@ typedef struct wan_attn_mask {
                                   the last row is at the last key */
 } wan_attn_mask;
 size_t wan_masked_attn_workspace(int batch, int heads_q, int heads_k, int seqlen_q, int seqlen_k, int head_dim,
-                                 int causal);
+                                 const wan_attn_mask* mask);
 int wan_masked_attn(wan_tensor q, wan_tensor k, wan_tensor v, wan_tensor out, int batch, int heads_q,
                     int heads_k, int seqlen_q, int seqlen_k, int head_dim, int dtype, float softmax_scale,
                     const wan_attn_mask* mask, void* workspace, size_t workspace_bytes, void* stream);

@@ -329,7 +329,7 @@ def test_less_scratch(W):
     """With the scratch of the C call cut short the keys are split less far; without any, not at all."""
     N, lib = W._native, W._native.lib()
     q, k, v, _ = _make(1, 1, 3000, 8, 2, 128, BF, 21)
-    need = lib.wan_masked_attn_workspace(1, 8, 2, 1, 3000, 128, 0)
+    need = lib.wan_masked_attn_workspace(1, 8, 2, 1, 3000, 128, None)
     assert need > 0
     want, tol = _reference(q, k, v, 0.1)
     ws = torch.empty(need, dtype=torch.uint8, device=DEV)

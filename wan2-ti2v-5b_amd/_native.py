@@ -70,7 +70,7 @@ SIGNATURES = {
     "wan_rope": (_I, [_T, _P, _I, _I, _I, _I, _P, _P, _P]),
     "wan_rms_norm": (_I, [_T, _P, _I, _I, _I, _I, _P, _F, _P, _P, _P, _P]),
     "wan_rms_norm_qk": (_I, [_T, _T, _P, _I, _I, _I, _I, _P, _F, _P, _P, _P, _P]),
-    "wan_masked_attn_workspace": (_SZ, [_I] * 7),
+    "wan_masked_attn_workspace": (_SZ, [_I] * 6 + [ctypes.POINTER(WanAttnMask)]),
     "wan_masked_attn": (_I, [_T, _T, _T, _T, _I, _I, _I, _I, _I, _I, _I, _F, ctypes.POINTER(WanAttnMask), _P, _SZ, _P]),
     "wan_head_norm_rope": (_I, [_T, _T, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P, _F, _P, _P, _I, _I, _P, _I, _P]),
     "wan_flash_attn_qnorm": (_I, [_T, _T, _T, _T, _I, _I, _I, _I, _I, _P, _P, _P, _P, _F, _P, _P]),

@@ -513,9 +513,10 @@ int wan_rope(wan_tensor x, void* out, int batch, int seqlen, int heads, int head
 }
 
 size_t wan_masked_attn_workspace(int batch, int heads_q, int heads_k, int seqlen_q, int seqlen_k, int head_dim,
-                                 int causal) {
+                                 const wan_attn_mask* mask) {
   if (heads_k <= 0 || heads_q % heads_k != 0 || (head_dim != 64 && head_dim != 128)) return 0;
-  return masked_split_bytes(batch, heads_q, heads_k, seqlen_q, seqlen_k, head_dim, causal != 0);
+  return masked_split_bytes(batch, heads_q, heads_k, seqlen_q, seqlen_k, head_dim, mask && mask->causal,
+                            mask && mask->seqlen_k);
 }
 
 int wan_masked_attn(wan_tensor q, wan_tensor k, wan_tensor v, wan_tensor out, int batch, int heads_q, int heads_k,

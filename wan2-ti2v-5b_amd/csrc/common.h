@@ -116,13 +116,13 @@ struct MaskedArgs {
   const int32_t* q_start;    // [B] position of query row 0 (null: Lk - Lq)
   float* part;               // scratch of the key split (null: none)
   size_t part_bytes;
-  // set by the launcher (MaskedPlan): blocks of rows of a unit, units times parts, and the divisions by these
-  int pack, splits, part_rows, part_floats, blocks, ups;
-  FastDiv by_pack, by_splits, by_blocks, by_batch, by_group, by_rows, by_last_ups;
+  // set by the launcher (MaskedPlan): blocks of rows of a unit, units of a sample, units times parts, and the divisions by these
+  int pack, splits, part_rows, part_floats, blocks, head_groups, ups;
+  FastDiv by_pack, by_splits, by_blocks, by_heads, by_group, by_rows, by_last_ups;
 };
 constexpr int kUnitGroup = 32;    // units of a group in the order of the workgroups
 int launch_masked_attn(MaskedArgs a, int D, int dtype, hipStream_t s);
-size_t masked_split_bytes(int B, int Hq, int Hk, int Lq, int Lk, int D, bool causal);
+size_t masked_split_bytes(int B, int Hq, int Hk, int Lq, int Lk, int D, bool causal, bool ragged);
 // CU count of the current device (cached per device after the first query).
 int device_cu_count();
 

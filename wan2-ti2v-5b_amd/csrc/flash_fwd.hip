@@ -1142,14 +1142,14 @@ int launch_flash_fwd(const FlashArgs& a, hipStream_t s) {
   }
 }
 
-size_t masked_split_bytes(int B, int Hq, int Hk, int Lq, int Lk, int D, bool causal) {
+size_t masked_split_bytes(int B, int Hq, int Hk, int Lq, int Lk, int D, bool causal, bool ragged) {
   if (B <= 0 || Hq <= 0 || Hk <= 0 || Lq <= 0 || Lk <= 0) return 0;
-  return masked_plan(B, Hq, Hk, Lq, Lk, D, causal, device_cu_count(), SIZE_MAX).bytes;
+  return masked_plan(B, Hq, Hk, Lq, Lk, D, causal, ragged, device_cu_count(), SIZE_MAX).bytes;
 }
 
 int launch_masked_attn(MaskedArgs a, int D, int dtype, hipStream_t s) {
   if (a.B == 0 || a.Hq == 0 || a.Lq == 0) return 0;
-  const MaskedPlan p = masked_plan(a.B, a.Hq, a.Hk, a.Lq, a.Lk, D, a.causal, device_cu_count(),
+  const MaskedPlan p = masked_plan(a.B, a.Hq, a.Hk, a.Lq, a.Lk, D, a.causal, a.seqlen_k != nullptr, device_cu_count(),
                                    a.part != nullptr ? a.part_bytes : 0);
   if (p.blocks * p.splits > 0x7fffffff || p.out_rows > 0x7fffffff)
     return set_error(2, "masked_attn: %lld workgroups is too many", (long long)p.blocks * p.splits);
@@ -1157,13 +1157,14 @@ int launch_masked_attn(MaskedArgs a, int D, int dtype, hipStream_t s) {
   a.splits = p.splits;
   a.part_rows = p.part_rows;
   a.part_floats = p.part_floats;
-  const int64_t units = (int64_t)(a.Hq / p.pack) * a.B;
+  a.head_groups = a.Hq / p.pack;
+  const int64_t units = (int64_t)a.head_groups * a.B;
   a.blocks = (int)(p.blocks / units);
   a.ups = (int)(units * p.splits);
   a.by_pack = FastDiv(a.pack);
   a.by_splits = FastDiv(a.splits);
   a.by_blocks = FastDiv(a.blocks);
-  a.by_batch = FastDiv(a.B);
+  a.by_heads = FastDiv(a.head_groups);
   a.by_group = FastDiv(a.Hq / a.Hk);
   a.by_rows = FastDiv(a.Lq * a.pack);
   a.by_last_ups = FastDiv(a.ups % kUnitGroup != 0 ? a.ups % kUnitGroup : 1);

@@ -181,14 +181,13 @@ __device__ __forceinline__ int rows_max(int v) {
   return max(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16));
 }
 
-// The sample and heads of a unit.  The samples vary fastest: units that run together are then long and
-// short ones alike.
+// The sample and heads of a unit.  The heads vary fastest: workgroup i runs on XCD i % 8, and every XCD has units of
+// long and of short samples.
 struct MaskedUnit {
   int b, h0, hk;          // sample, first of the P query heads, their k/v head
   __device__ __forceinline__ MaskedUnit(const MaskedArgs& a, int unit) {
-    const int group = a.by_batch(unit);
-    b = uniform(unit - group * a.B);
-    h0 = uniform(group * a.pack);
+    b = uniform(a.by_heads(unit));
+    h0 = uniform((unit - b * a.head_groups) * a.pack);
     hk = uniform(a.by_group(h0));
   }
   // (the tile copies take their addresses from scalar registers)
@@ -607,12 +606,19 @@ __global__ __launch_bounds__(kStepWaves * 64, 1) void masked_step_kernel(const M
 // many rows: 32 a wave, on tiles of 64 keys that a workgroup's waves share
 // ---------------------------------------------------------------------------
 //
-// KG = 1: eight waves of rows (256).  KG = 2: four (128), the other four waves are the same rows on every
-// second tile; a block then takes half as many steps, which is what a launch with few, or unequally long,
-// blocks ends sooner by, for twice the tile copies.
+// KG = 1: all NW waves have rows of their own, eight (256 rows, a workgroup a CU) for 128 channels, four for 64, of
+// which two workgroups fit a CU, so that one's start and end overlap the other's tiles.  (us, 64 channels, eight /
+// four: 512 text tokens with bias 19.4 / 15.4, 2049 tokens with prefixes 38.2 / 32.1, 24 heads of 4096 tokens
+// 140 / 127, 2 x 7854 causal 441 / 452.  With 128 channels four have LDS for rings of two tiles: 24 heads of 4096
+// tokens 216 / 202, 2 x 7854 causal 722 / 745.)
+// KG = 2: eight waves, four of rows (128), the other four the same rows on every second tile; a block then takes
+// half as many steps, which is what a launch with few, or unequally long, blocks ends sooner by, for twice the
+// tile copies (us, KG 1 / 2: 2 x 1024 tokens causal, 16 over 4 heads of 128 channels 30.0 / 20.6, 24 heads of 1000
+// tokens 29.5 / 21.4, of 64 channels 17.7 / 15.8; 2 x 7854 causal 722 / 787).
 
-constexpr int kBlockWaves = kAttnWaves, kBlockKeys = kTileKeys;
-constexpr int kBlockWindow = 8128;      // bias entries of a workgroup
+constexpr int kBlockKeys = kTileKeys;
+template <int HD> constexpr int kBlockWaves = HD == 128 ? 8 : 4;
+constexpr int kWaveWindow = 1016;       // bias entries of a workgroup, for each of its waves
 
 // The order of the workgroups: units (and their parts) in groups of kUnitGroup, in a group the last rows of all
 // its units first.  Under a causal mask those see the most keys, so that the short blocks fill the end of the
@@ -750,18 +756,18 @@ struct BlockCore {
   }
 };
 
-template <typename T, int HD, bool CAP, bool BIAS, int KG>
-__global__ __launch_bounds__(kBlockWaves * 64, 2) void masked_block_kernel(const MaskedArgs a) {
+template <typename T, int HD, bool CAP, bool BIAS, int NW, int KG>
+__global__ __launch_bounds__(NW * 64, 2) void masked_block_kernel(const MaskedArgs a) {
   typedef typename Elem<T>::x8 X8;
   typedef typename Elem<T>::x4 X4;
-  constexpr int kRowWaves = kBlockWaves / KG, BM = kRowWaves * 32, BK = kBlockKeys, kTile = BK * HD;
+  constexpr int kRowWaves = NW / KG, BM = kRowWaves * 32, BK = kBlockKeys, kTile = BK * HD;
   // Rings of four k and v tiles and a barrier every second tile.  With KG = 1, as in the unmasked kernel, an
   // even step issues the copies of the next pair of tiles and the odd one waits for them; with KG = 2 a step
   // is a pair of tiles.
   __shared__ __attribute__((aligned(1024))) bf16 k_lds[4][kTile];
   __shared__ __attribute__((aligned(1024))) bf16 v_lds[4][kTile];
-  __shared__ float window[BIAS ? kBlockWindow : 1];
-  __shared__ int ends[2][kBlockWaves];
+  __shared__ float window[BIAS ? NW * kWaveWindow : 1];
+  __shared__ int ends[2][NW];
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -780,8 +786,8 @@ __global__ __launch_bounds__(kBlockWaves * 64, 2) void masked_block_kernel(const
   }
   // What the first tile needs goes out before it is known which tiles these rows see: without documents, and
   // not split, they begin with tile 0 (if they see any).
-  MaskedCopy<HD, BK, kBlockWaves, false> kc;
-  MaskedCopy<HD, BK, kBlockWaves, true> vc;
+  MaskedCopy<HD, BK, NW, false> kc;
+  MaskedCopy<HD, BK, NW, true> vc;
   kc.init(static_cast<const T*>(a.k.ptr) + blk.b * a.k.sb + blk.hk * a.k.sh, a.k.st, wave, lane);
   vc.init(static_cast<const T*>(a.v.ptr) + blk.b * a.v.sb + blk.hk * a.v.sh, a.v.st, wave, lane);
   const bool early = a.doc_starts == nullptr && a.splits == 1 && a.Lk > 0;
@@ -799,7 +805,7 @@ __global__ __launch_bounds__(kBlockWaves * 64, 2) void masked_block_kernel(const
   __syncthreads();
   int first = ends[0][0], end = ends[1][0];
 #pragma unroll
-  for (int n = 1; n < kBlockWaves; ++n) {
+  for (int n = 1; n < NW; ++n) {
     first = min(first, ends[0][n]);
     end = max(end, ends[1][n]);
   }
@@ -828,7 +834,7 @@ __global__ __launch_bounds__(kBlockWaves * 64, 2) void masked_block_kernel(const
     BiasWindow win;
     int p_first = 0, p_last = 0;       // positions of the workgroup's rows
     if constexpr (BIAS) {
-      win.init(kBlockWindow, a.pack);
+      win.init(NW * kWaveWindow, a.pack);
       const int at = MaskedUnit::uniform(w.m.p - w.i);
       p_first = at + a.by_pack(row0);
       p_last = at + a.by_pack(min(row0 + BM, rows) - 1);
@@ -851,7 +857,7 @@ __global__ __launch_bounds__(kBlockWaves * 64, 2) void masked_block_kernel(const
         if (!win.holds(k0 - p_last, k0 + KG * BK - 1 - p_first)) {
           __syncthreads();
           win.load(a, blk.h0, k0 - p_last, (int64_t)(nt - u0 + KG - 1) * BK + (p_last - p_first), window, threadIdx.x,
-                   kBlockWaves * 64);
+                   NW * 64);
           __syncthreads();
         }
       }
@@ -953,7 +959,7 @@ __global__ __launch_bounds__(kBlockWaves * 64, 2) void masked_block_kernel(const
   if (bad)
     attend_wave<T, HD, CAP, BIAS, 1>(a, blk, w, max(range.first * (BK / kWaveKeys), w.first / kWaveKeys) + kg,
                                      min(range.end * (BK / kWaveKeys), (w.end - 1) / kWaveKeys + 1), KG, share,
-                                     window + wave * (kBlockWindow / kBlockWaves), kBlockWindow / kBlockWaves, lane, c.o,
+                                     window + wave * (kWaveWindow), kWaveWindow, lane, c.o,
                                      c.m_run, c.l_run);
   if constexpr (KG == 2) {
     // The second four waves leave what they have to the first: the rows lie in the same lanes.
@@ -1060,12 +1066,12 @@ __global__ __launch_bounds__(256) void masked_merge_kernel(const MaskedArgs a, i
     v += f * o;
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  const int group = a.by_batch(unit), b = unit - group * a.B, qi = a.by_pack(r);
+  const int b = a.by_heads(unit), h0 = (unit - b * a.head_groups) * a.pack, qi = a.by_pack(r);
   X4 y;
 #pragma unroll
   for (int e = 0; e < 4; ++e) y[e] = (T)(v[e] * inv);
   *reinterpret_cast<X4*>(static_cast<T*>(a.o) + b * a.o_sb + (int64_t)qi * a.o_st +
-                         (group * a.pack + r - qi * a.pack) * a.o_sh + 4 * lane) = y;
+                         (h0 + r - qi * a.pack) * a.o_sh + 4 * lane) = y;
 }
 
 // ---------------------------------------------------------------------------
@@ -1077,10 +1083,10 @@ int launch_masked(MaskedArgs a, const MaskedPlan& p, hipStream_t s) {
   const dim3 grid((unsigned)(p.blocks * p.splits));
   if (p.block_rows == 32)
     hipLaunchKernelGGL((masked_step_kernel<T, HD, CAP, BIAS>), grid, dim3(kStepWaves * 64), 0, s, a);
-  else if (p.block_rows == 128)
-    hipLaunchKernelGGL((masked_block_kernel<T, HD, CAP, BIAS, 2>), grid, dim3(kBlockWaves * 64), 0, s, a);
+  else if (p.key_groups == 2)
+    hipLaunchKernelGGL((masked_block_kernel<T, HD, CAP, BIAS, 8, 2>), grid, dim3(512), 0, s, a);
   else
-    hipLaunchKernelGGL((masked_block_kernel<T, HD, CAP, BIAS, 1>), grid, dim3(kBlockWaves * 64), 0, s, a);
+    hipLaunchKernelGGL((masked_block_kernel<T, HD, CAP, BIAS, kBlockWaves<HD>, 1>), grid, dim3(kBlockWaves<HD> * 64), 0, s, a);
   if (p.splits > 1)
     hipLaunchKernelGGL((masked_merge_kernel<T, HD>), dim3((unsigned)((p.out_rows + 1024 / HD - 1) / (1024 / HD))),
                        dim3(256), 0, s, a,

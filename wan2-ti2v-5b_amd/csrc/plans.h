@@ -66,19 +66,32 @@ constexpr float kExactCap = 256.f;
 // holds the distances of 32 keys and 3 positions for.
 constexpr int kMaxPack = 28;
 
-// How a call is run: `pack` query heads of one k/v head are rows of a block, `blocks` blocks of block_rows
+// How a call is run: `pack` query heads of one k/v head are rows of a unit, in `blocks` blocks of block_rows
 // rows, each as `splits` workgroups over a part of its keys.  A part's result: part_rows rows of D fp32,
 // their maxima and their sums.
 struct MaskedPlan {
-  int pack, block_rows, splits, part_rows, part_floats;
+  int pack, block_rows, key_groups, splits, part_rows, part_floats;
   int64_t blocks, out_rows;
   size_t bytes;
 };
-// Up to this many rows of a unit go by tiles of 32 rows, whose waves split the keys, more by blocks of 256.
+// Up to this many rows of a unit go by tiles of 32 rows, whose waves split the keys, more by blocks.
 constexpr int kStepRows = 32;
 constexpr int kMaskedMaxSplits = 64;
-constexpr float kBlockUs = 3.f, kMaskedMergeUs = 4.f;
-inline MaskedPlan masked_plan(int B, int Hq, int Hk, int Lq, int Lk, int D, bool causal, int cus, size_t scratch) {
+// The kernels of blocks: rows, key groups, workgroups that a CU holds, and what a step of theirs (a tile, with two
+// key groups two) takes in us where as many run as a CU holds, and where one runs alone.
+struct MaskedKernel {
+  int D, rows, key_groups, slots;
+  float step, alone, block;     // block: what one takes besides
+};
+constexpr MaskedKernel kMaskedKernels[] = {{128, 256, 1, 1, 1.9f, 1.9f, 3.f},
+                                           {128, 128, 2, 1, 2.2f, 2.05f, 4.f},
+                                           {64, 128, 1, 2, 1.1f, 0.75f, 3.f},
+                                           {64, 128, 2, 1, 1.3f, 1.25f, 4.f}};
+// What the last blocks take where not all run at once; and a split: the merge launch, and the parts' way through
+// memory.
+constexpr float kTailUs = 5.f, kMaskedMergeUs = 7.f, kMaskedPartUs = 4.f / 1e7f;
+inline MaskedPlan masked_plan(int B, int Hq, int Hk, int Lq, int Lk, int D, bool causal, bool ragged, int cus,
+                              size_t scratch) {
   MaskedPlan p{};
   const int group = Hq / Hk;
   p.pack = group < kMaxPack ? group : kMaxPack;
@@ -87,8 +100,9 @@ inline MaskedPlan masked_plan(int B, int Hq, int Hk, int Lq, int Lk, int D, bool
   p.out_rows = rows * units;
   const int nt = (Lk + kTileKeys - 1) / kTileKeys;
   // blocks of `block_rows` rows, `n` parts: whether the scratch holds them
-  auto layout = [&](int block_rows, int n) {
+  auto layout = [&](int block_rows, int key_groups, int n) {
     p.block_rows = block_rows;
+    p.key_groups = key_groups;
     p.blocks = (rows + block_rows - 1) / block_rows * units;
     p.part_rows = (int)(rows < block_rows ? rows : block_rows);
     p.part_floats = (p.part_rows * (D + 2) + 3) / 4 * 4;
@@ -97,38 +111,53 @@ inline MaskedPlan masked_plan(int B, int Hq, int Hk, int Lq, int Lk, int D, bool
     return p.bytes <= scratch;
   };
   if (rows <= kStepRows) {
-    int64_t n = 2 * (int64_t)cus / units;
+    // One workgroup a CU; with key lengths of their own three, if they are left 20 tiles each, so that the long
+    // samples do not end last (us with 1 / 2 / 4 / 6 / 8 parts, 16 samples of 8 k/v heads: 8192 keys 115 / 99 / 110 /
+    // 106 / 112, 2048 to 8192 keys 105 / 78 / 74 / 69 / 71, 1000 keys 20 / 20 / 25 / 30 / 31).
+    int64_t n = cus / units;
     if (n > (nt + 3) / 4) n = (nt + 3) / 4;
+    if (ragged && n < 3 * (int64_t)cus / units) {
+      const int64_t more = 3 * (int64_t)cus / units < nt / 20 ? 3 * (int64_t)cus / units : nt / 20;
+      if (more > n) n = more;
+    }
     if (n > kMaskedMaxSplits) n = kMaskedMaxSplits;
     if (n < 1) n = 1;
-    while (!layout(32, (int)n)) --n;
+    while (!layout(32, 1, (int)n)) --n;
     return p;
   }
-  // Of a block's tiles (nt at most) a workgroup, one a CU, takes `step` us each, with 128 rows for each pair, and
-  // kBlockUs besides.  Without a causal mask the blocks run in rounds; with one the longest come first and the
-  // launch ends with the longest or when the sum of all is done.  A split costs the merge launch and the
-  // parts' way through memory.
+  // Of a block's tiles (nt at most) `mean` are seen.  Without a causal mask the blocks run in rounds; with one the
+  // longest come first and the launch ends with the longest or when the sum of all is done.  Over 26 random sizes
+  // the choice was 4% slower than the best of both kernels and 1 to 8 parts, 20% at worst.
   const float mean = causal ? nt - 0.5f * ((Lq < Lk ? Lq : Lk) / kTileKeys) : (float)nt;
   float best = 0.f;
-  int best_rows = 0, best_n = 1;
-  for (int block_rows = 256; block_rows >= 128; block_rows /= 2) {
-    const int pair = 256 / block_rows;
-    const float step = D == 128 ? (pair == 1 ? 1.9f : 2.05f) : (pair == 1 ? 1.15f : 1.25f);
-    for (int n = 1; n <= kMaskedMaxSplits && (n == 1 || n * 4 * pair <= nt); ++n) {
-      if (!layout(block_rows, n)) break;
-      const float longest = step * ((nt + n * pair - 1) / (n * pair)) + kBlockUs;
-      const float sum = p.blocks * n * (step * (mean / (n * pair) + 0.5f) + kBlockUs) / cus;
-      const float rounds = (float)((p.blocks * n + cus - 1) / cus) * longest;
-      float us = causal ? (sum > longest ? sum : longest) : rounds;
-      if (n > 1) us += kMaskedMergeUs + p.bytes * (2.f / 1e7f);
-      if (best_rows == 0 || us < 0.95f * best) {
+  const MaskedKernel* chosen = nullptr;
+  int chosen_n = 1;
+  for (const MaskedKernel& k : kMaskedKernels) {
+    if (k.D != D) continue;
+    const int tiles = k.key_groups;       // of a step
+    for (int n = 1; n <= kMaskedMaxSplits && (n == 1 || n * 4 * tiles <= nt); ++n) {
+      if (!layout(k.rows, k.key_groups, n)) break;
+      const float wgs = (float)p.blocks * n, slots = (float)cus * k.slots;
+      // a block of all tiles (where the causal ones get shorter the rest runs at a higher clock)
+      auto whole = [&](float step) { return (causal ? 0.8f : 1.f) * step * ((nt + n * tiles - 1) / (n * tiles)) + k.block; };
+      float us;
+      if (causal) {
+        const float sum = wgs * (k.step * (mean / (n * tiles) + 0.5f) + k.block) / slots;
+        const float longest = whole(wgs <= cus ? k.alone : k.step);
+        us = (sum > longest ? sum : longest) + (wgs > slots ? kTailUs : 0.f);
+      } else {
+        const float full = (float)(int64_t)(wgs / slots), rest = wgs - full * slots;
+        us = full * whole(k.step) + (rest > 0.f ? whole(rest <= cus ? k.alone : k.step) : 0.f);
+      }
+      if (n > 1) us += kMaskedMergeUs + p.bytes * kMaskedPartUs;
+      if (chosen == nullptr || us < 0.97f * best) {
         best = us;
-        best_rows = block_rows;
-        best_n = n;
+        chosen = &k;
+        chosen_n = n;
       }
     }
   }
-  layout(best_rows, best_n);
+  layout(chosen->rows, chosen->key_groups, chosen_n);
   return p;
 }
 

@@ -408,7 +408,7 @@ void masked_attn(const OperatorHandle& op, DispatchKeySet ks, Stack* stack) {
             D = (int)q.size(3);
   const Site s(q);
   Tensor out = s.rows(q);
-  const Scratch ws(s, wan_masked_attn_workspace(B, Hq, Hk, Lq, Lk, D, causal));
+  const Scratch ws(s, wan_masked_attn_workspace(B, Hq, Hk, Lq, Lk, D, &m));
   check("wan_masked_attn", wan_masked_attn(t4(q), t4(k), t4(v), t4(out), B, Hq, Hk, Lq, Lk, D, type, c.real(3), &m,
                                            ws.ptr(), ws.n, s.stream()));
   c.give(std::move(out));

@@ -433,7 +433,7 @@ def masked_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, softmax_scale
     mask = N.WanAttnMask(int(causal), float(softcap), ptr(bias), reach, ptr(doc_starts), docs, ptr(prefix_lens),
                          ptr(seqlen_k), ptr(q_start))
     with torch.cuda.device(q.device):
-        n = lib.wan_masked_attn_workspace(B, Hq, Hk, Lq, Lk, D, int(causal))
+        n = lib.wan_masked_attn_workspace(B, Hq, Hk, Lq, Lk, D, mask)
         ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
         N.check("wan_masked_attn", lib.wan_masked_attn(
             N.tensor4(q), N.tensor4(k), N.tensor4(v), N.tensor4(out), B, Hq, Hk, Lq, Lk, D, _DTYPES[q.dtype],
