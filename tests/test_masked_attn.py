@@ -211,6 +211,39 @@ def test_documents(W, Lq, Lk, Hq, Hk, docs, causal, prefix, dtype, D):
            prefix=None if prefix is None else _ints(prefix + [[1, 0, 20, 21]]))
 
 
+MANY = {"large": [0, 700, 701, 1500, 1560, 2300], "one_large": [0, 20, 40, 2400], "late": [900, 1000, 2999], "even": list(range(0, 3000, 30)),
+        "odd": [0] + [7 + 13 * i + (i % 5) * 2 for i in range(200)], "outside": [-50, 0, 1200, 3000, 3500], "same": [0, 5, 5, 5, 1400, 1400]}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D,causal", [(64, False), (64, True), (128, False), (128, True)])
+@pytest.mark.parametrize("which", list(MANY))
+@pytest.mark.parametrize("Lq,Hq,Hk", [(3000, 2, 1), (1800, 1, 1)])
+def test_many_documents(W, Lq, Hq, Hk, which, D, causal):
+    """Blocks of rows that begin with the large documents and hold runs of small ones; more than 64 documents; starts
+    outside the keys; empty documents."""
+    q, k, v, bias = _make(2, Lq, 3000, Hq, Hk, D, BF, 6, 60 if which == "odd" else None)
+    first = MANY[which]
+    other = sorted((37 * i * i + 11 * i) % 3000 for i in range(len(first)))
+    _check(W, q, k, v, D ** -0.5, causal=causal, bias=bias, docs=_ints([first, other]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("starts", [[2500, 100, 50, 1700], [2 ** 31 - 1, 0, -(2 ** 31), 5], [0, 3000, 10, 2000]])
+def test_documents_out_of_order_write_every_row_in_bounds(W, starts):
+    N, lib = W._native, W._native.lib()
+    for D, Lq in ((64, 3000), (128, 2777)):
+        q, k, v, _ = _make(1, Lq, 3000, 2, 1, D, BF, 8)
+        whole = torch.full((1, Lq + 2, 2, D), float("nan"), device=DEV, dtype=BF)
+        out, docs = whole[:, 1:-1], _ints([starts])
+        mask = N.WanAttnMask(doc_starts=docs.data_ptr(), docs=4)
+        N.check("wan_masked_attn", lib.wan_masked_attn(
+            N.tensor4(q), N.tensor4(k), N.tensor4(v), N.tensor4(out), 1, 2, 1, Lq, 3000, D, 0, 0.1, ctypes.byref(mask), None, 0,
+            torch.cuda.current_stream().cuda_stream))
+        assert torch.isfinite(out.float()).all() and (out.float().abs() <= v.float().abs().max()).all()
+        assert whole[:, 0].isnan().all() and whole[:, -1].isnan().all()
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("prefix", [[0, 0], [1, 700], [64, 333], [2 ** 31 - 1, -5]])
 @pytest.mark.parametrize("Lq,Lk,Hq,Hk", [(700, 700, 4, 2), (1, 90, 4, 4), (100, 700, 2, 1)])

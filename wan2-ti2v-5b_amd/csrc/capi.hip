@@ -516,7 +516,8 @@ size_t wan_masked_attn_workspace(int batch, int heads_q, int heads_k, int seqlen
                                  const wan_attn_mask* mask) {
   if (heads_k <= 0 || heads_q % heads_k != 0 || (head_dim != 64 && head_dim != 128)) return 0;
   return masked_split_bytes(batch, heads_q, heads_k, seqlen_q, seqlen_k, head_dim, mask && mask->causal,
-                            mask && mask->seqlen_k);
+                            mask && mask->seqlen_k,
+                            mask && mask->doc_starts ? mask->docs : 0);
 }
 
 int wan_masked_attn(wan_tensor q, wan_tensor k, wan_tensor v, wan_tensor out, int batch, int heads_q, int heads_k,

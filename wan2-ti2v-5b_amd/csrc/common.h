@@ -118,11 +118,12 @@ struct MaskedArgs {
   size_t part_bytes;
   // set by the launcher (MaskedPlan): blocks of rows of a unit, units of a sample, units times parts, and the divisions by these
   int pack, splits, part_rows, part_floats, blocks, head_groups, ups;
+  bool by_docs;               // blocks begin and end with the large documents
   FastDiv by_pack, by_splits, by_blocks, by_heads, by_group, by_rows, by_last_ups;
 };
 constexpr int kUnitGroup = 32;    // units of a group in the order of the workgroups
 int launch_masked_attn(MaskedArgs a, int D, int dtype, hipStream_t s);
-size_t masked_split_bytes(int B, int Hq, int Hk, int Lq, int Lk, int D, bool causal, bool ragged);
+size_t masked_split_bytes(int B, int Hq, int Hk, int Lq, int Lk, int D, bool causal, bool ragged, int docs);
 // CU count of the current device (cached per device after the first query).
 int device_cu_count();
 

@@ -1142,19 +1142,21 @@ int launch_flash_fwd(const FlashArgs& a, hipStream_t s) {
   }
 }
 
-size_t masked_split_bytes(int B, int Hq, int Hk, int Lq, int Lk, int D, bool causal, bool ragged) {
+size_t masked_split_bytes(int B, int Hq, int Hk, int Lq, int Lk, int D, bool causal, bool ragged, int docs) {
   if (B <= 0 || Hq <= 0 || Hk <= 0 || Lq <= 0 || Lk <= 0) return 0;
-  return masked_plan(B, Hq, Hk, Lq, Lk, D, causal, ragged, device_cu_count(), SIZE_MAX).bytes;
+  return masked_plan(B, Hq, Hk, Lq, Lk, D, causal, ragged, docs, device_cu_count(), SIZE_MAX).bytes;
 }
 
 int launch_masked_attn(MaskedArgs a, int D, int dtype, hipStream_t s) {
   if (a.B == 0 || a.Hq == 0 || a.Lq == 0) return 0;
-  const MaskedPlan p = masked_plan(a.B, a.Hq, a.Hk, a.Lq, a.Lk, D, a.causal, a.seqlen_k != nullptr, device_cu_count(),
+  const MaskedPlan p = masked_plan(a.B, a.Hq, a.Hk, a.Lq, a.Lk, D, a.causal, a.seqlen_k != nullptr,
+                                   a.doc_starts != nullptr ? a.docs : 0, device_cu_count(),
                                    a.part != nullptr ? a.part_bytes : 0);
   if (p.blocks * p.splits > 0x7fffffff || p.out_rows > 0x7fffffff)
     return set_error(2, "masked_attn: %lld workgroups is too many", (long long)p.blocks * p.splits);
   a.pack = p.pack;
   a.splits = p.splits;
+  a.by_docs = p.by_docs;
   a.part_rows = p.part_rows;
   a.part_floats = p.part_floats;
   a.head_groups = a.Hq / p.pack;

@@ -120,10 +120,14 @@ struct MaskedRow {
   int p, lo, hi;      // position; keys seen: [lo, hi), empty rows [0, 0)
 };
 
+__device__ __forceinline__ int first_position(const MaskedArgs& a, int b) {
+  const int start = a.q_start != nullptr ? a.q_start[b] : a.Lk - a.Lq;
+  return max(min(start, kMaxPosition), -kMaxPosition);
+}
+
 __device__ __forceinline__ MaskedRow masked_row(const MaskedArgs& a, int b, int i) {
   MaskedRow r;
-  const int start = a.q_start != nullptr ? a.q_start[b] : a.Lk - a.Lq;
-  r.p = max(min(start, kMaxPosition), -kMaxPosition) + i;
+  r.p = first_position(a, b) + i;
   int len = a.Lk;
   if (a.seqlen_k != nullptr) len = min(max(a.seqlen_k[b], 0), a.Lk);
   int lo = 0, hi = len, prefix = 0;
@@ -214,26 +218,25 @@ struct TileRange {
 // ---------------------------------------------------------------------------
 
 // The softmax's arithmetic on one lane's scores.  CAP: capped by a tanh.  BIAS: a table entry added.
-// Without either the scores stay as the MFMA leaves them and the scale is folded into the exponent.
+// map() leaves a value that times `factor` (plus the bias) is the score in units of log2(e), up to a constant
+// of all scores: without CAP the MFMA's own; with it
+//   cap tanh(y) = cap + 2 cap (-1 / (1 + e^2y)),
+// the last bracket, off by 2^-22 at most, which up to caps of 256 is less than the rounding of the softmax
+// weights; beyond (`precise`), tanh(y) itself, for small y by the series y - y^3/3 + 2 y^5/15.
+// The factor is folded into the exponent; with BIAS value and entry are joined first.
 template <bool CAP, bool BIAS>
 struct ScoreMap {
-  float sl2;            // scale * log2(e)
-  float cap2, k;        // cap * log2(e); 2 log2(e) scale / cap, if precise scale / cap
+  float factor;         // scale * log2(e); 2 cap * log2(e), if precise cap * log2(e)
+  float k;              // CAP: 2 log2(e) scale / cap, if precise scale / cap
   bool precise;
 
   __device__ __forceinline__ void init(const MaskedArgs& a) {
-    sl2 = a.scale * kLog2e;
-    cap2 = a.cap * kLog2e;
     precise = a.cap > kExactCap;
+    factor = CAP ? (precise ? a.cap * kLog2e : 2.f * kLog2e * a.cap) : a.scale * kLog2e;
     k = CAP ? (precise ? a.scale / a.cap : 2.f * kLog2e * a.scale / a.cap) : 0.f;
   }
-  // Scores in units of log2(e), without bias (without cap and bias: as they are).
-  // tanh(y) = 1 - 2 / (1 + e^2y): off by 2^-22 of the cap at most, which up to caps of 256 is less than the
-  // rounding of the softmax weights; beyond (`precise`), small y go by the series y - y^3/3 + 2 y^5/15.
   __device__ __forceinline__ float one(float s) const {
-    if constexpr (CAP) return fmaf(-2.f * cap2, __builtin_amdgcn_rcpf(1.f + fast_exp2(s * k)), cap2);
-    else if constexpr (BIAS) return s * sl2;
-    else return s;
+    return CAP ? __builtin_amdgcn_rcpf(-1.f - fast_exp2(s * k)) : s;
   }
   template <bool SMALL = false>       // SMALL: the cap is known not to be `precise`
   __device__ __forceinline__ void map(f32x16& s) const {
@@ -243,20 +246,22 @@ struct ScoreMap {
         const float y = s[r] * k, y2 = y * y;
         const float far = fmaf(-2.f, __builtin_amdgcn_rcpf(1.f + fast_exp2(y * (2.f * kLog2e))), 1.f);
         const float near = fmaf(y * y2, fmaf(y2, 2.f / 15.f, -1.f / 3.f), y);
-        s[r] = cap2 * (fabsf(y) < 0.1f ? near : far);
+        s[r] = fabsf(y) < 0.1f ? near : far;
       }
-    } else {
+    } else if (CAP) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = one(s[r]);
     }
   }
-  // exponent of a score against the reference point m
+  // with BIAS: the mapped value and the table entry of its distance
+  __device__ __forceinline__ float add(float s, float entry) const { return fmaf(s, factor, entry); }
+  // the weight of a score against the reference point m
   __device__ __forceinline__ float weight(float s, float m) const {
-    if constexpr (CAP || BIAS) return fast_exp2(s - m);
-    else return fast_exp2(fmaf(s, sl2, -m));
+    if constexpr (BIAS) return fast_exp2(s - m);
+    else return fast_exp2(fmaf(s, factor, -m));
   }
   // a max of scores in the units of m
-  __device__ __forceinline__ float top(float s) const { return CAP || BIAS ? s : s * sl2; }
+  __device__ __forceinline__ float top(float s) const { return BIAS ? s : s * factor; }
 };
 
 // A bias entry in units of log2(e).  What is finite stays finite: a table may hold the type's lowest value
@@ -483,7 +488,7 @@ __device__ __forceinline__ void attend_wave(const MaskedArgs& a, const MaskedUni
     if constexpr (BIAS) {
       const float* e0 = window + w.g * win.per + (kt + 4 * hh - w.m.p - win.w0);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) s[e] += e0[8 * (e >> 2) + (e & 3)];
+      for (int e = 0; e < 16; ++e) s[e] = map.add(s[e], e0[8 * (e >> 2) + (e & 3)]);
     }
     const bool masked = kt < w.all_lo || kt + kWaveKeys > w.all_hi;
     if (masked) mask_scores(s, kt, hh, w.m);
@@ -620,20 +625,88 @@ constexpr int kBlockKeys = kTileKeys;
 template <int HD> constexpr int kBlockWaves = HD == 128 ? 8 : 4;
 constexpr int kWaveWindow = 1016;       // bias entries of a workgroup, for each of its waves
 
-// The order of the workgroups: units (and their parts) in groups of kUnitGroup, in a group the last rows of all
-// its units first.  Under a causal mask those see the most keys, so that the short blocks fill the end of the
-// launch.  Workgroup i runs on XCD i % 8: the blocks of a unit share one L2 where the units of a group are a
+// The order of the workgroups: units (and their parts) in groups of kUnitGroup, in a group the first blocks of all its
+// units first.  Those are the rows that see the most keys (the last ones, which under a causal mask do, or the
+// longest document's), so that the short blocks fill the end of the launch.  Workgroup i runs on XCD i % 8: the blocks of a unit share one L2 where the units of a group are a
 // multiple of 8, and where they are fewer each unit's long and short blocks spread evenly over the XCDs.
 struct BlockOrder {
-  int up, rb;
+  int up, at;
   __device__ __forceinline__ BlockOrder(const MaskedArgs& a, int id) {
     const int group = a.by_blocks(id / kUnitGroup), in = id - group * (kUnitGroup * a.blocks);
     // (the last group may be smaller)
     const bool whole = (group + 1) * kUnitGroup <= a.ups;
     const int size = whole ? kUnitGroup : a.ups - group * kUnitGroup;
-    const int at = whole ? in / kUnitGroup : a.by_last_ups(in);
+    at = whole ? in / kUnitGroup : a.by_last_ups(in);
     up = group * kUnitGroup + (in - at * size);
-    rb = a.blocks - 1 - at;
+  }
+};
+
+// Inclusive scans over the wave's 64 lanes, `none` where there is nothing to the left.
+template <typename F>
+__device__ __forceinline__ int wave_scan(int v, int none, F op) {
+  v = op(v, __builtin_amdgcn_update_dpp(none, v, 0x111, 0xf, 0xf, false));    // 1, 2, 4, 8 lanes on, in 16
+  v = op(v, __builtin_amdgcn_update_dpp(none, v, 0x112, 0xf, 0xf, false));
+  v = op(v, __builtin_amdgcn_update_dpp(none, v, 0x114, 0xf, 0xf, false));
+  v = op(v, __builtin_amdgcn_update_dpp(none, v, 0x118, 0xf, 0xf, false));
+  v = op(v, __builtin_amdgcn_update_dpp(none, v, 0x142, 0xa, 0xf, false));    // lane 15's, 47's to the next 16
+  v = op(v, __builtin_amdgcn_update_dpp(none, v, 0x143, 0xc, 0xf, false));    // lane 31's to the upper 32
+  return v;
+}
+
+// The rows of block `at` of a sample's unit: of blocks of BM rows, the last ones first; with documents (not
+// split) of blocks that begin where a document of 2 BM rows or more begins or ends.  A block over the border of
+// two such reads the keys of both, half of its waves idle in each.  (7854 tokens in documents of 374, 1080, 2244
+// and 4156, 24 heads of 128 channels: 366 -> 278 us.)  Runs of smaller documents stay together.  The longest
+// run's blocks come first.  Rows before the first document are a run too, and a row is in one block whatever
+// the starts hold.  Blocks past the last one have no rows.
+struct RowBlock {
+  int first, end;
+  __device__ __forceinline__ RowBlock(const MaskedArgs& a, int b, int at, int BM, int lane) {
+    const int rows = a.Lq * a.pack;
+    if (!a.by_docs) {
+      first = (a.blocks - 1 - at) * BM;
+      end = min(first + BM, rows);
+      return;
+    }
+    const int start = first_position(a, b);
+    const int32_t* d = a.doc_starts + (int64_t)b * a.docs;
+    int begun = 0;            // rows of the runs before these 64
+    first = end = rows;
+    for (int j0 = 0; j0 <= a.docs; j0 += 64) {
+      // this lane's document (0: none yet, j: the j-th) ends in front of row `to`
+      const int j = j0 + lane;
+      int to = rows;
+      if (j < a.docs) {
+        const int64_t q = (int64_t)d[j] - start;
+        to = (int)(min(max(q, (int64_t)0), (int64_t)a.Lq) * a.pack);
+      }
+      to = max(begun, wave_scan(to, 0, [](int x, int y) { return max(x, y); }));
+      int from = __shfl_up(to, 1);
+      if (lane == 0) from = begun;
+      const bool large = to - from >= 2 * BM;
+      const bool large_before = __shfl_up((int)large, 1) != 0;
+      const uint64_t heads = __builtin_amdgcn_ballot_w64(lane == 0 || large || large_before);
+      const bool head = heads >> lane & 1;
+      const uint64_t later = lane == 63 ? 0 : heads >> (lane + 1);
+      const int run_last = later != 0 ? lane + __builtin_ctzll(later) : 63;       // the run's last lane
+      const int run_end = __shfl(to, run_last), size = run_end - from;
+      const int count = head ? (size + BM - 1) / BM : 0;
+      const int total = __builtin_amdgcn_readlane(wave_scan(count, 0, [](int x, int y) { return x + y; }), 63);
+      if (at < total) {
+        int before = 0;       // blocks of the longer runs
+        for (uint64_t m = heads; m != 0; m &= m - 1) {
+          const int other = __builtin_ctzll(m), s = __builtin_amdgcn_readlane(size, other);
+          if (s > size || (s == size && other < lane)) before += __builtin_amdgcn_readlane(count, other);
+        }
+        const int mine = __builtin_ctzll(__builtin_amdgcn_ballot_w64(head && before <= at && at < before + count));
+        const int k = at - __builtin_amdgcn_readlane(before, mine), n = __builtin_amdgcn_readlane(count, mine);
+        first = __builtin_amdgcn_readlane(from, mine) + (n - 1 - k) * BM;
+        end = min(first + BM, __builtin_amdgcn_readlane(run_end, mine));
+        return;
+      }
+      at -= total;
+      begun = __builtin_amdgcn_readlane(to, 63);
+    }
   }
 };
 
@@ -772,11 +845,12 @@ __global__ __launch_bounds__(NW * 64, 2) void masked_block_kernel(const MaskedAr
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n32 = lane & 31, hh = lane >> 5;
-  const int rows = a.Lq * a.pack;
   const BlockOrder order(a, blockIdx.x);
   const int unit = a.by_splits(order.up), part = order.up - unit * a.splits;
-  const int row0 = MaskedUnit::uniform(order.rb * BM);
   const MaskedUnit blk(a, unit);
+  const RowBlock block_rows(a, blk.b, order.at, BM, lane);
+  const int row0 = MaskedUnit::uniform(block_rows.first), rows = MaskedUnit::uniform(block_rows.end);
+  if (row0 >= rows) return;
   const int kg = wave / kRowWaves, wrow0 = row0 + (wave - kg * kRowWaves) * 32;
   const bool live = wrow0 < rows;      // (a wave without rows copies its share and meets the barriers)
   WaveRows w(a, blk.b, wrow0, rows, lane);
@@ -837,7 +911,7 @@ __global__ __launch_bounds__(NW * 64, 2) void masked_block_kernel(const MaskedAr
       win.init(NW * kWaveWindow, a.pack);
       const int at = MaskedUnit::uniform(w.m.p - w.i);
       p_first = at + a.by_pack(row0);
-      p_last = at + a.by_pack(min(row0 + BM, rows) - 1);
+      p_last = at + a.by_pack(rows - 1);
     }
     // whether the wave's rows see any key of tile u
     auto seen = [&](int u) {
@@ -872,8 +946,8 @@ __global__ __launch_bounds__(NW * 64, 2) void masked_block_kernel(const MaskedAr
           const float* bias = window + w.g * win.per + (kt + 4 * hh - w.m.p - win.w0);
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            c0[e] += bias[8 * (e >> 2) + (e & 3)];
-            c1[e] += bias[32 + 8 * (e >> 2) + (e & 3)];
+            c0[e] = c.map.add(c0[e], bias[8 * (e >> 2) + (e & 3)]);
+            c1[e] = c.map.add(c1[e], bias[32 + 8 * (e >> 2) + (e & 3)]);
           }
         }
         if (masked) {

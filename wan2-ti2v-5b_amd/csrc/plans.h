@@ -73,6 +73,7 @@ struct MaskedPlan {
   int pack, block_rows, key_groups, splits, part_rows, part_floats;
   int64_t blocks, out_rows;
   size_t bytes;
+  bool by_docs;       // blocks begin and end with the documents of two blocks or more (not split)
 };
 // Up to this many rows of a unit go by tiles of 32 rows, whose waves split the keys, more by blocks.
 constexpr int kStepRows = 32;
@@ -90,15 +91,15 @@ constexpr MaskedKernel kMaskedKernels[] = {{128, 256, 1, 1, 1.9f, 1.9f, 3.f},
 // What the last blocks take where not all run at once; and a split: the merge launch, and the parts' way through
 // memory.
 constexpr float kTailUs = 5.f, kMaskedMergeUs = 7.f, kMaskedPartUs = 4.f / 1e7f;
-inline MaskedPlan masked_plan(int B, int Hq, int Hk, int Lq, int Lk, int D, bool causal, bool ragged, int cus,
-                              size_t scratch) {
+inline MaskedPlan masked_plan(int B, int Hq, int Hk, int Lq, int Lk, int D, bool causal, bool ragged, int docs,
+                              int cus, size_t scratch) {
   MaskedPlan p{};
   const int group = Hq / Hk;
   p.pack = group < kMaxPack ? group : kMaxPack;
   while (group % p.pack != 0) --p.pack;
   const int64_t rows = (int64_t)Lq * p.pack, units = (int64_t)(Hq / p.pack) * B;
   p.out_rows = rows * units;
-  const int nt = (Lk + kTileKeys - 1) / kTileKeys;
+  int nt = (Lk + kTileKeys - 1) / kTileKeys;
   // blocks of `block_rows` rows, `n` parts: whether the scratch holds them
   auto layout = [&](int block_rows, int key_groups, int n) {
     p.block_rows = block_rows;
@@ -109,6 +110,15 @@ inline MaskedPlan masked_plan(int B, int Hq, int Hk, int Lq, int Lk, int D, bool
     p.splits = n;
     p.bytes = n > 1 ? (size_t)p.blocks * p.part_floats * sizeof(float) * n : 0;
     return p.bytes <= scratch;
+  };
+  // A run of documents ends in a block of its own: there is one for each large document and between two of them,
+  // and at every 64th of all (the kernel goes through 64 at a time).
+  auto by_documents = [&] {
+    if (docs <= 0 || p.splits > 1) return;
+    const int64_t plain = (rows + p.block_rows - 1) / p.block_rows;
+    const int64_t runs = plain + 2 + docs / 64;
+    p.blocks = (plain + (runs < docs + 1 ? runs : docs + 1)) * units;
+    p.by_docs = true;
   };
   if (rows <= kStepRows) {
     // One workgroup a CU; with key lengths of their own three, if they are left 20 tiles each, so that the long
@@ -125,6 +135,8 @@ inline MaskedPlan masked_plan(int B, int Hq, int Hk, int Lq, int Lk, int D, bool
     while (!layout(32, 1, (int)n)) --n;
     return p;
   }
+  // (documents are of unequal length: about twice the mean of them)
+  if (docs > 0 && 2 * (nt / docs + 1) < nt) nt = 2 * (nt / docs + 1);
   // Of a block's tiles (nt at most) `mean` are seen.  Without a causal mask the blocks run in rounds; with one the
   // longest come first and the launch ends with the longest or when the sum of all is done.  Over 26 random sizes
   // the choice was 4% slower than the best of both kernels and 1 to 8 parts, 20% at worst.
@@ -158,6 +170,7 @@ inline MaskedPlan masked_plan(int B, int Hq, int Hk, int Lq, int Lk, int D, bool
     }
   }
   layout(chosen->rows, chosen->key_groups, chosen_n);
+  by_documents();
   return p;
 }
 
