@@ -138,7 +138,7 @@ typedef struct wan_attn_mask {
   int docs;
   const int32_t* prefix_lens;  /* [batch], with doc_starts [batch, docs]; causal only */
   const int32_t* seqlen_k;     /* [batch]; NULL: seqlen_k for all */
-  const int32_t* q_start;      /* [batch], within +- 2^30; NULL: seqlen_k - seqlen_q (the argument's), so that
+  const int32_t* q_start;      /* [batch], within +- 2^29; NULL: seqlen_k - seqlen_q (the argument's), so that
                                   the last row is at the last key */
 } wan_attn_mask;
 size_t wan_masked_attn_workspace(int batch, int heads_q, int heads_k, int seqlen_q, int seqlen_k, int head_dim,

@@ -218,7 +218,7 @@ MANY = {"large": [0, 700, 701, 1500, 1560, 2300], "one_large": [0, 20, 40, 2400]
 @pytest.mark.gpu
 @pytest.mark.parametrize("D,causal", [(64, False), (64, True), (128, False), (128, True)])
 @pytest.mark.parametrize("which", list(MANY))
-@pytest.mark.parametrize("Lq,Hq,Hk", [(3000, 2, 1), (1800, 1, 1)])
+@pytest.mark.parametrize("Lq,Hq,Hk", [(3000, 2, 1), (1800, 1, 1), (7, 4, 2), (1, 3, 1)])
 def test_many_documents(W, Lq, Hq, Hk, which, D, causal):
     """Blocks of rows that begin with the large documents and hold runs of small ones; more than 64 documents; starts
     outside the keys; empty documents."""

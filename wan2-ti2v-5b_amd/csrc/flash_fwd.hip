@@ -1152,7 +1152,8 @@ int launch_masked_attn(MaskedArgs a, int D, int dtype, hipStream_t s) {
   const MaskedPlan p = masked_plan(a.B, a.Hq, a.Hk, a.Lq, a.Lk, D, a.causal, a.seqlen_k != nullptr,
                                    a.doc_starts != nullptr ? a.docs : 0, device_cu_count(),
                                    a.part != nullptr ? a.part_bytes : 0);
-  if (p.blocks * p.splits > 0x7fffffff || p.out_rows > 0x7fffffff)
+  // (a launch has fewer than 2^32 threads: 512 a block, D / 4 a row of the merge)
+  if (p.blocks * p.splits >= (int64_t(1) << 23) || (p.splits > 1 && p.out_rows >= (int64_t(1) << 27)))
     return set_error(2, "masked_attn: %lld workgroups is too many", (long long)p.blocks * p.splits);
   a.pack = p.pack;
   a.splits = p.splits;

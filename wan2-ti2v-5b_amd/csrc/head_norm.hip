@@ -43,22 +43,45 @@ __device__ __forceinline__ void store8(T* p, const float x[8]) {
   __builtin_nontemporal_store(v, reinterpret_cast<V*>(p));
 }
 
+// The sum over a head's lanes, in all of them: neighbours, pairs and halves of 8 by lane permutations, 16 by
+// rotations.
+template <int C>
+__device__ __forceinline__ float lane_move(float v) {
+  return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), C, 0xf, 0xf, true));
+}
+template <int LPH>
+__device__ __forceinline__ float head_sum(float v) {
+  if constexpr (LPH == 8) {
+    v += lane_move<0xb1>(v);      // the neighbour of 2
+    v += lane_move<0x4e>(v);      // the other pair of 4
+    v += lane_move<0x141>(v);     // the other four, mirrored
+  } else {
+    v += lane_move<0x128>(v);
+    v += lane_move<0x124>(v);
+    v += lane_move<0x122>(v);
+    v += lane_move<0x121>(v);
+    if constexpr (LPH == 32) v += __shfl_xor(v, 16);
+  }
+  return v;
+}
+
 // LPH lanes a head, NCH heads a lane.
 template <typename T, int LPH, int NCH>
 __global__ __launch_bounds__(256) void head_norm_kernel(const HeadNormArgs a) {
   typedef typename Vec8<T>::type V __attribute__((aligned(16)));
   const int lane = threadIdx.x & 63;
-  const int64_t wave = row_block(a.grid_x) * 4 + (threadIdx.x >> 6);
-  const int64_t group = wave / a.waves_per_token;     // tokens of one wave
-  const int part = (int)(wave - group * a.waves_per_token);
+  const int wave = (int)(row_block(a.grid_x) * 4) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (wave >= a.waves) return;
+  const int group = a.by_waves(wave);                 // tokens of one wave
+  const int part = wave - group * a.waves_per_token;
   const int slot = lane / LPH, chunk = lane % LPH;
-  const int64_t tok = (group << a.token_shift) + (slot >> a.slot_shift);
+  const int64_t tok = ((int64_t)group << a.token_shift) + (slot >> a.slot_shift);
   const bool live = tok < (int64_t)a.B * a.L && chunk * 8 < a.D;
   const int heads = a.Hq + a.Hk;
   const int per_step = 1 << a.slot_shift;             // heads of a token that a wave works on at once
   const int h0 = part * (per_step * NCH) + (slot & (per_step - 1));
   const int d0 = chunk * 8;
-  const int b = live ? (int)(tok / a.L) : 0, l = live ? (int)(tok - (int64_t)b * a.L) : 0;
+  const int b = live ? a.by_tokens((int)tok) : 0, l = live ? (int)tok - b * a.L : 0;
 
   V xv[NCH];
 #pragma unroll
@@ -95,10 +118,10 @@ __global__ __launch_bounds__(256) void head_norm_kernel(const HeadNormArgs a) {
       }
     }
   }
-  float gq[8] = {}, gk[8] = {};
+  V gq = V{}, gk = V{};
   if (chunk * 8 < a.D) {
-    load8(static_cast<const T*>(a.gamma_q) + d0, gq);
-    load8(static_cast<const T*>(a.gamma_k) + d0, gk);
+    gq = *reinterpret_cast<const V*>(static_cast<const T*>(a.gamma_q) + d0);
+    gk = *reinterpret_cast<const V*>(static_cast<const T*>(a.gamma_k) + d0);
   }
 
 #pragma unroll
@@ -110,11 +133,10 @@ __global__ __launch_bounds__(256) void head_norm_kernel(const HeadNormArgs a) {
       u[j] = (float)xv[i][j];
       ss = fmaf(u[j], u[j], ss);
     }
-#pragma unroll
-    for (int m = LPH / 2; m >= 1; m >>= 1) ss += __shfl_xor(ss, m);
+    ss = head_sum<LPH>(ss);
     const float inv = 1.0f / sqrtf(ss / (float)a.D + a.eps);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) u[j] = u[j] * inv * (h < a.Hq ? gq[j] : gk[j]);
+    for (int j = 0; j < 8; ++j) u[j] = u[j] * inv * (float)(h < a.Hq ? gq[j] : gk[j]);
     if (a.cos != nullptr) {
       if (a.interleaved) {
         if (turned) {
@@ -152,7 +174,11 @@ __global__ __launch_bounds__(256) void head_norm_kernel(const HeadNormArgs a) {
 template <typename T, int LPH, int NCH>
 int launch(HeadNormArgs a, hipStream_t s) {
   const HeadNormPlan p = head_norm_plan((int64_t)a.B * a.L, a.Hq + a.Hk, LPH, NCH);
+  if (p.waves > 0x7ff00000) return set_error(2, "head_norm: %lld waves is too many", (long long)p.waves);
+  a.waves = (int)p.waves;
   a.waves_per_token = p.waves_per_token;
+  a.by_waves = FastDiv(p.waves_per_token);
+  a.by_tokens = FastDiv(a.L);
   a.slot_shift = p.slot_shift;
   a.token_shift = p.token_shift;
   const RowGrid g = row_grid((p.waves + 3) / 4, 256);

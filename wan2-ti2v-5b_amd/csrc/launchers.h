@@ -78,7 +78,8 @@ struct HeadNormArgs {
   bool interleaved;     // pairs (2j, 2j + 1), else (j, j + P)
   // set by the launcher (HeadNormPlan)
   unsigned grid_x;
-  int waves_per_token, slot_shift, token_shift;
+  int waves, waves_per_token, slot_shift, token_shift;
+  FastDiv by_waves, by_tokens;
 };
 int launch_head_norm(const HeadNormArgs& a, int dtype, hipStream_t s);
 

@@ -57,9 +57,9 @@ inline SplitPlan split_plan(int B, int H, int Lq, int keys, int cus, size_t scra
 // the attention under masks (masked_attn.h)
 // ---------------------------------------------------------------------------
 
-// Sizes up to this (keys, query rows of a sample over their heads) and positions of the first query row
-// within +- this keep every position and distance in 32 bits.
-constexpr int kMaxPosition = (1 << 30) - 1;
+// Positions of the first query row within +- this, as many keys, and twice as many rows keep every position and
+// distance in 32 bits.
+constexpr int kMaxPosition = (1 << 29) - 1;
 // Caps above this take the form of the tanh that is exact for small arguments too.
 constexpr float kExactCap = 256.f;
 // Query heads that are rows beside each other, at most: as many as a wave's share of the bias entries (1016)
