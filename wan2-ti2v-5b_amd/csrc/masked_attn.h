@@ -218,39 +218,74 @@ struct TileRange {
 // ---------------------------------------------------------------------------
 
 // The softmax's arithmetic on one lane's scores.  CAP: capped by a tanh.  BIAS: a table entry added.
-// map() leaves a value that times `factor` (plus the bias) is the score in units of log2(e), up to a constant
-// of all scores: without CAP the MFMA's own; with it
-//   cap tanh(y) = cap + 2 cap (-1 / (1 + e^2y)),
-// the last bracket, off by 2^-22 at most, which up to caps of 256 is less than the rounding of the softmax
-// weights; beyond (`precise`), tanh(y) itself, for small y by the series y - y^3/3 + 2 y^5/15.
+// map() leaves a value that times `factor` (plus the bias) is the score in units of log2(e): without CAP the MFMA's
+// own, with it tanh(y), y = s scale / cap.  Where all of the wave's |y| are at most 1/4 that is the series
+// y - y^3/3 + 2 y^5/15 - 17 y^7/315, off by 2^-23 at most, in five operations; its usual form 1 - 2 / (1 + e^2y) takes
+// an exponential and a reciprocal, of a quarter of the rate, beside the softmax's own (us a tile of 256 rows, of 128 /
+// 64 channels: 2.35 / 1.77 -> 2.22 / 1.68; uncapped 1.90 / 1.15).  That form is off by 2^-22, which up to caps of 256 is less than the rounding of the softmax weights; beyond,
+// |y| up to 1/4 go by the series beside it too.
 // The factor is folded into the exponent; with BIAS value and entry are joined first.
 template <bool CAP, bool BIAS>
 struct ScoreMap {
-  float factor;         // scale * log2(e); 2 cap * log2(e), if precise cap * log2(e)
-  float k;              // CAP: 2 log2(e) scale / cap, if precise scale / cap
-  bool precise;
+  float factor;         // scale * log2(e); cap * log2(e)
+  float c1, c3, c5, c7; // CAP: the series in s
+  float k;              // 2 log2(e) scale / cap
+  float small, exact;   // the |s| up to which the series holds, and (for large caps) is taken of any score
 
   __device__ __forceinline__ void init(const MaskedArgs& a) {
-    precise = a.cap > kExactCap;
-    factor = CAP ? (precise ? a.cap * kLog2e : 2.f * kLog2e * a.cap) : a.scale * kLog2e;
-    k = CAP ? (precise ? a.scale / a.cap : 2.f * kLog2e * a.scale / a.cap) : 0.f;
+    factor = (CAP ? a.cap : a.scale) * kLog2e;
+    c1 = CAP ? a.scale / a.cap : 0.f;
+    const float sq = c1 * c1;
+    c3 = c1 * sq * (-1.f / 3.f);
+    c5 = c1 * sq * sq * (2.f / 15.f);
+    c7 = c1 * sq * sq * sq * (-17.f / 315.f);
+    k = 2.f * kLog2e * c1;
+    small = CAP && c1 < 1e4f ? 0.25f / c1 : -1.f;        // (with more the series' factors might overflow)
+    exact = a.cap > kExactCap ? small : -1.f;
   }
-  __device__ __forceinline__ float one(float s) const {
-    return CAP ? __builtin_amdgcn_rcpf(-1.f - fast_exp2(s * k)) : s;
+  __device__ __forceinline__ float form(float s) const {
+    return fmaf(2.f, __builtin_amdgcn_rcpf(-1.f - fast_exp2(s * k)), 1.f);
   }
-  template <bool SMALL = false>       // SMALL: the cap is known not to be `precise`
-  __device__ __forceinline__ void map(f32x16& s) const {
-    if (CAP && !SMALL && precise) {
+  // What is left of the map after begin(): the series, or nothing.
+  struct Rest {
+    float c1, c3, c5, c7;
+    __device__ __forceinline__ float operator()(float s) const {
+      const float z = s * s;
+      return s * fmaf(z, fmaf(z, fmaf(z, c7, c5), c3), c1);
+    }
+  };
+  // The first half of the map, of N x 16 scores: where the series holds for all of the wave, nothing.
+  template <int N>
+  __device__ __forceinline__ Rest begin(f32x16* const (&s)[N]) const {
+    Rest rest{c1, c3, c5, c7};
+    if constexpr (CAP) {
+      float top = fabsf((*s[0])[0]);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const float y = s[r] * k, y2 = y * y;
-        const float far = fmaf(-2.f, __builtin_amdgcn_rcpf(1.f + fast_exp2(y * (2.f * kLog2e))), 1.f);
-        const float near = fmaf(y * y2, fmaf(y2, 2.f / 15.f, -1.f / 3.f), y);
-        s[r] = fabsf(y) < 0.1f ? near : far;
+      for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf((*s[n])[r]));
+      if (__builtin_amdgcn_ballot_w64(!(top <= small)) != 0) {
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const float v = (*s[n])[r], near = rest(v), far = form(v);
+            (*s[n])[r] = fabsf(v) <= exact ? near : far;
+          }
+        rest = Rest{1.f, 0.f, 0.f, 0.f};
       }
-    } else if (CAP) {
+    }
+    return rest;
+  }
+  // N x 16 scores
+  template <int N>
+  __device__ __forceinline__ void map(f32x16* const (&s)[N]) const {
+    if constexpr (CAP) {
+      const Rest rest = begin<N>(s);
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = one(s[r]);
+      for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) (*s[n])[r] = rest((*s[n])[r]);
     }
   }
   // with BIAS: the mapped value and the table entry of its distance
@@ -484,7 +519,7 @@ __device__ __forceinline__ void attend_wave(const MaskedArgs& a, const MaskedUni
     f32x16 s = {};
 #pragma unroll
     for (int ks = 0; ks < HD / 16; ++ks) s = Elem<T>::mfma(op.k_frag(Kt, ks, 0), op.qf[ks], s);
-    map.map(s);
+    map.template map<1>({&s});
     if constexpr (BIAS) {
       const float* e0 = window + w.g * win.per + (kt + 4 * hh - w.m.p - win.w0);
 #pragma unroll
@@ -766,9 +801,11 @@ struct BlockCore {
     return acc[0] + acc[1];
   }
 
-  // The same with the MFMAs of the next tile's scores in between, k fragments read one step ahead.
-  __device__ __forceinline__ float qk_exp(const bf16* Kt, f32x16& n0, f32x16& n1, const f32x16& c0, const f32x16& c1,
-                                          X8 pb[4]) const {
+  // The same with the MFMAs of the next tile's scores in between, k fragments read one step ahead.  MAP: what is left
+  // of the scores' map too (`bias`: this lane's entry of the tile's first key).
+  template <bool MAP>
+  __device__ __forceinline__ float qk_exp(const bf16* Kt, f32x16& n0, f32x16& n1, f32x16& c0, f32x16& c1, X8 pb[4],
+                                          const typename ScoreMap<CAP, BIAS>::Rest& rest, const float* bias) const {
     float acc0 = 0.f, acc1 = 0.f;
     X8 a0 = op.k_frag(Kt, 0, 0), a1 = op.k_frag(Kt, 0, 32);
 #pragma unroll
@@ -780,6 +817,19 @@ struct BlockCore {
       }
       n0 = Elem<T>::mfma(a0, op.qf[ks], ks == 0 ? f32x16{} : n0);
       n1 = Elem<T>::mfma(a1, op.qf[ks], ks == 0 ? f32x16{} : n1);
+      if constexpr (MAP && (CAP || BIAS)) {
+#pragma unroll
+        for (int r = kEach * ks; r < kEach * (ks + 1); ++r) {
+          if (CAP) {
+            c0[r] = rest(c0[r]);
+            c1[r] = rest(c1[r]);
+          }
+          if constexpr (BIAS) {
+            c0[r] = map.add(c0[r], bias[8 * (r >> 2) + (r & 3)]);
+            c1[r] = map.add(c1[r], bias[32 + 8 * (r >> 2) + (r & 3)]);
+          }
+        }
+      }
 #pragma unroll
       for (int r = kEach * ks; r < kEach * (ks + 1); r += 2) {
         weigh(c0, r, m_run, pb, acc0);
@@ -940,25 +990,31 @@ __global__ __launch_bounds__(NW * 64, 2) void masked_block_kernel(const MaskedAr
       const bf16 *Kn = k_lds[(u + KG) & 3], *Vt = v_lds[u & 3];
       X8 pb[4];
       if (here) {
-        c.map.template map<LEAN>(c0);
-        c.map.template map<LEAN>(c1);
-        if constexpr (BIAS) {
-          const float* bias = window + w.g * win.per + (kt + 4 * hh - w.m.p - win.w0);
+        const float* bias = nullptr;
+        if constexpr (BIAS) bias = window + w.g * win.per + (kt + 4 * hh - w.m.p - win.w0);
+        float rs;
+        if constexpr (LEAN) {
+          const auto rest = c.map.template begin<2>({&c0, &c1});
+          rs = c.template qk_exp<true>(Kn, n0, n1, c0, c1, pb, rest, bias);
+        } else {
+          c.map.template map<2>({&c0, &c1});
+          if constexpr (BIAS) {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            c0[e] = c.map.add(c0[e], bias[8 * (e >> 2) + (e & 3)]);
-            c1[e] = c.map.add(c1[e], bias[32 + 8 * (e >> 2) + (e & 3)]);
+            for (int e = 0; e < 16; ++e) {
+              c0[e] = c.map.add(c0[e], bias[8 * (e >> 2) + (e & 3)]);
+              c1[e] = c.map.add(c1[e], bias[32 + 8 * (e >> 2) + (e & 3)]);
+            }
           }
+          if (masked) {
+            mask_scores(c0, kt, hh, w.m);
+            mask_scores(c1, kt + 32, hh, w.m);
+          }
+          if (fresh) {
+            c.m_run = fmaxf(-FLT_MAX, c.tile_top(c0, c1));
+            fresh = false;
+          }
+          rs = next ? c.template qk_exp<false>(Kn, n0, n1, c0, c1, pb, {}, nullptr) : c.exp_tile(c0, c1, pb);
         }
-        if (masked) {
-          mask_scores(c0, kt, hh, w.m);
-          mask_scores(c1, kt + 32, hh, w.m);
-        }
-        if (!LEAN && fresh) {
-          c.m_run = fmaxf(-FLT_MAX, c.tile_top(c0, c1));
-          fresh = false;
-        }
-        const float rs = next ? c.qk_exp(Kn, n0, n1, c0, c1, pb) : c.exp_tile(c0, c1, pb);
         c.finish(c0, c1, rs, pb);
       } else if (next) {
         c.qk(Kn, n0, n1);
@@ -999,9 +1055,10 @@ __global__ __launch_bounds__(NW * 64, 2) void masked_block_kernel(const MaskedAr
     if (seen(kg)) {
       c.qk(k_lds[kg], sa0, sa1);
       // The first reference point, where every row sees the whole tile.  (With a bias it needs the mapped scores:
-      // one that lies above all of a row's would leave it no weights.)
-      if (!BIAS && lean_lo <= 0 && base + (kg + 1) * BK <= w.all_hi && !(CAP && c.map.precise)) {
-        c.m_run = c.map.top(c.map.one(pair_max(fmaxf(max16(sa0), max16(sa1)))));
+      // one that lies above all of a row's would leave it no weights.  The tanh grows with the score.)
+      if (!BIAS && lean_lo <= 0 && base + (kg + 1) * BK <= w.all_hi) {
+        const float top = pair_max(fmaxf(max16(sa0), max16(sa1)));
+        c.m_run = c.map.top(CAP ? c.map.form(top) : top);
         fresh = !(c.m_run >= -FLT_MAX && c.m_run <= FLT_MAX);
         if (__builtin_amdgcn_ballot_w64(fresh) != 0) c.m_run = -FLT_MAX;
         fresh = __builtin_amdgcn_ballot_w64(fresh) != 0;
@@ -1009,7 +1066,7 @@ __global__ __launch_bounds__(NW * 64, 2) void masked_block_kernel(const MaskedAr
     }
     __syncthreads();      // every wave is done with the first tiles of k before they are overwritten
     for (int u = 0; u < nt; u += 2 * KG) {
-      while (u >= lean_lo && u < lean_hi && !fresh && !(CAP && c.map.precise) &&
+      while (u >= lean_lo && u < lean_hi && !fresh &&
              (!BIAS || win.holds(base + u * BK - p_last, base + (u + 2 * KG) * BK - 1 - p_first))) {
         step(std::true_type{}, u, sa0, sa1, sb0, sb1);
         step(std::true_type{}, u + KG, sb0, sb1, sa0, sa1);
