@@ -2,14 +2,17 @@
  * wan_attn.h — C ABI of the MI355X (gfx950) attention path of the
  * Wan2.2-TI2V-5B DiT: flash self-attention, cross-attention with per-sample
  * key lengths, QK-RMSNorm and 3D-RoPE (standalone and fused into the
- * attention kernels).
+ * attention kernels); and for packed batches, text encoders and single tokens
+ * beside it, norms of single heads with the rotation by position, and attention
+ * under masks.
  *
  * Conventions
  *   - Tensors are bf16 device pointers in the DiT projection layout
  *     [batch, token, head, head_dim] (a view of [batch, token, dim]) described
  *     by wan_tensor: element strides of batch, token and head; head_dim is
- *     contiguous.  head_dim must be 128, the data pointer 16-byte aligned and
- *     every stride a multiple of 8 elements.
+ *     contiguous.  head_dim must be 128 (wan_masked_attn: 64 or 128,
+ *     wan_head_norm_rope: a multiple of 8 up to 256; both take other types too),
+ *     the data pointer 16-byte aligned and every stride a multiple of 8 elements.
  *   - RoPE tables are fp32 [seqlen, head_dim/2] cos and sin (the layout of
  *     _rope_tables, models/fast_dit.py:548-558, without the unit dims).
  *   - Outputs and workspaces are allocated by the caller; the library never
@@ -124,13 +127,13 @@ int wan_flash_attn_qnorm_ws(wan_tensor q, wan_tensor k, wan_tensor v, wan_tensor
  *   out_i  = softmax over the keys seen of s_i, times v;  zeros where no key is seen, or all of them at -inf
  * v rows of keys that a row does not see do not reach it, whatever they hold.  The arrays are on the device
  * and int32: values outside their ranges are clamped, doc_starts that do not ascend give other documents,
- * never a read out of range.  `workspace` is optional scratch of wan_masked_attn_workspace() bytes, 256-byte
- * aligned (for this mask; 0: not needed): with it calls whose rows leave compute units idle split their keys over them,
- * with fewer bytes less far.
+ * never a read out of range.  `out` does not overlap the inputs.  `workspace` is optional scratch of
+ * wan_masked_attn_workspace() bytes, 256-byte aligned (for this mask; 0: not needed): with it calls whose rows leave
+ * compute units idle split their keys over them, with fewer bytes less far.
  */
 typedef struct wan_attn_mask {
   int causal;
-  float softcap;               /* 0: none; finite, >= 0 */
+  float softcap;               /* 0: none; at most 1e30 */
   const float* bias;           /* [heads_q, 2 bias_reach + 1] fp32; finite or -inf (hides the key) */
   int bias_reach;              /* R: distances beyond it have the bias of R */
   const int32_t* doc_starts;   /* [batch, docs] first positions, ascending; a document ends where the next

@@ -35,6 +35,8 @@ def test_abi_refusals(W):
                            (dict(k=N.WanTensor(P, 4096, -512, 64)), 1, "negative"),
                            (dict(v=N.WanTensor(P, 4096, 1 << 24, 64)), 2, "token stride"),
                            (dict(softcap=-1.0), 1, "softcap"), (dict(softcap=float("nan")), 1, "softcap"),
+                           (dict(softcap=1e31), 1, "softcap"), (dict(softcap=float("inf")), 1, "softcap"),
+                           (dict(Lq=(1 << 29) + 1), 2, "2^29"),
                            (dict(bias=P, bias_reach=-1), 1, "bias_reach"), (dict(doc_starts=P), 1, "docs"),
                            (dict(prefix_lens=P), 1, "prefix_lens"), (dict(seqlen_k=P + 2), 1, "aligned"),
                            (dict(ws=P + 16, n=1 << 20), 1, "workspace")):
@@ -174,6 +176,26 @@ def test_sizes(W, Lq, Lk, Hq, Hk, causal, D, dtype):
 def test_cap(W, Lq, Lk, Hq, Hk, cap, dtype, D):
     q, k, v, _ = _make(1, Lq, Lk, Hq, Hk, D, dtype, 7, spread=3.0)
     _check(W, q, k, v, 2 * D ** -0.5, causal=True, cap=cap)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,D", [(BF, 128), (HF, 64)])
+@pytest.mark.parametrize("cap", [1e9, 1e30])
+@pytest.mark.parametrize("Lq,Lk", [(1, 300), (300, 333)])
+def test_caps_beyond_every_score_change_nothing(W, Lq, Lk, cap, dtype, D):
+    """With |s| < 2^10 the cap takes s (s / cap)^2 / 3 < 2^-29 of a score: the uncapped result, to its rounding."""
+    q, k, v, _ = _make(1, Lq, Lk, 4, 2, D, dtype, 8, spread=3.0)
+    want, tol = _reference(q, k, v, 2 * D ** -0.5)
+    assert ((W.ops.masked_attn(q, k, v, 2 * D ** -0.5, softcap=cap).double() - want).abs() <= tol).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cap", [1e-38, 1e-30, 1e-6])
+@pytest.mark.parametrize("Lq,Lk", [(1, 300), (300, 333)])
+def test_caps_far_below_the_scores(W, Lq, Lk, cap):
+    q, k, v, _ = _make(1, Lq, Lk, 4, 2, 128, BF, 9, spread=3.0)
+    q[:, :, 0] = 0
+    _check(W, q, k, v, 2 * 128 ** -0.5, cap=cap)
 
 
 @pytest.mark.gpu

@@ -538,15 +538,15 @@ int wan_masked_attn(wan_tensor q, wan_tensor k, wan_tensor v, wan_tensor out, in
   if (batch == 0 || heads_q == 0 || seqlen_q == 0) return WAN_OK;
   if (heads_k == 0 || heads_q % heads_k != 0)
     return set_error(WAN_ERR_INVALID, "%s: %d query heads are no multiple of %d k/v heads", fn, heads_q, heads_k);
-  if (seqlen_k > (1 << 29) || (int64_t)seqlen_q * (heads_q / heads_k) > (1 << 30))
-    return set_error(WAN_ERR_UNSUPPORTED, "%s: %d keys exceed 2^29 or %d rows of %d heads 2^30", fn, seqlen_k,
-                     seqlen_q, heads_q / heads_k);
+  if (seqlen_k > (1 << 29) || seqlen_q > (1 << 29) || (int64_t)seqlen_q * (heads_q / heads_k) > (1 << 30))
+    return set_error(WAN_ERR_UNSUPPORTED, "%s: %d keys or %d queries exceed 2^29, or the queries of %d heads 2^30", fn,
+                     seqlen_k, seqlen_q, heads_q / heads_k);
   if ((rc = check_tensor(fn, "q", q, batch, seqlen_q, heads_q))) return rc;
   if ((rc = check_tensor(fn, "k", k, batch, seqlen_k, heads_k))) return rc;
   if ((rc = check_tensor(fn, "v", v, batch, seqlen_k, heads_k))) return rc;
   if ((rc = check_tensor(fn, "out", out, batch, seqlen_q, heads_q))) return rc;
-  if (!(m.softcap >= 0.f) || !(m.softcap < INFINITY))
-    return set_error(WAN_ERR_INVALID, "%s: softcap=%g, must be finite and >= 0", fn, (double)m.softcap);
+  if (!(m.softcap >= 0.f) || !(m.softcap <= 1e30f))
+    return set_error(WAN_ERR_INVALID, "%s: softcap=%g, must be in [0, 1e30]", fn, (double)m.softcap);
   if (m.bias && (m.bias_reach < 0 || m.bias_reach > (1 << 29)))
     return set_error(WAN_ERR_INVALID, "%s: bias_reach=%d must be in [0, 2^29]", fn, m.bias_reach);
   if (m.doc_starts && m.docs <= 0) return set_error(WAN_ERR_INVALID, "%s: docs=%d, must be > 0", fn, m.docs);

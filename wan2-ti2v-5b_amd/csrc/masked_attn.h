@@ -222,15 +222,16 @@ struct TileRange {
 // own, with it tanh(y), y = s scale / cap.  Where all of the wave's |y| are at most 1/4 that is the series
 // y - y^3/3 + 2 y^5/15 - 17 y^7/315, off by 2^-23 at most, in five operations; its usual form 1 - 2 / (1 + e^2y) takes
 // an exponential and a reciprocal, of a quarter of the rate, beside the softmax's own (us a tile of 256 rows, of 128 /
-// 64 channels: 2.35 / 1.77 -> 2.22 / 1.68; uncapped 1.90 / 1.15).  That form is off by 2^-22, which up to caps of 256 is less than the rounding of the softmax weights; beyond,
-// |y| up to 1/4 go by the series beside it too.
+// 64 channels: 2.35 / 1.77 -> 2.22 / 1.68; uncapped 1.90 / 1.15).  That form is off by 2^-22, which up to caps of 256 is
+// less than the rounding of the softmax weights; beyond, |y| up to 1/4 go by the series beside it too.  (So the scores
+// of the rows beside it may move a capped row's by 2^-22 of the cap; nothing else of a row depends on another.)
 // The factor is folded into the exponent; with BIAS value and entry are joined first.
 template <bool CAP, bool BIAS>
 struct ScoreMap {
   float factor;         // scale * log2(e); cap * log2(e)
   float c1, c3, c5, c7; // CAP: the series in s
   float k;              // 2 log2(e) scale / cap
-  float small, exact;   // the |s| up to which the series holds, and (for large caps) is taken of any score
+  float small, exact;   // the |s| up to which all go by the series; the |y| up to which (for large caps) each does
 
   __device__ __forceinline__ void init(const MaskedArgs& a) {
     factor = (CAP ? a.cap : a.scale) * kLog2e;
@@ -239,9 +240,9 @@ struct ScoreMap {
     c3 = c1 * sq * (-1.f / 3.f);
     c5 = c1 * sq * sq * (2.f / 15.f);
     c7 = c1 * sq * sq * sq * (-17.f / 315.f);
-    k = 2.f * kLog2e * c1;
-    small = CAP && c1 < 1e4f ? 0.25f / c1 : -1.f;        // (with more the series' factors might overflow)
-    exact = a.cap > kExactCap ? small : -1.f;
+    k = fminf(2.f * kLog2e * c1, FLT_MAX);
+    small = CAP && c1 > 1e-5f && c1 < 1e4f ? 0.25f / c1 : -1.f;      // (where c7 neither overflows nor vanishes)
+    exact = a.cap > kExactCap ? 0.25f : -1.f;
   }
   __device__ __forceinline__ float form(float s) const {
     return fmaf(2.f, __builtin_amdgcn_rcpf(-1.f - fast_exp2(s * k)), 1.f);
@@ -269,8 +270,9 @@ struct ScoreMap {
         for (int n = 0; n < N; ++n)
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
-            const float v = (*s[n])[r], near = rest(v), far = form(v);
-            (*s[n])[r] = fabsf(v) <= exact ? near : far;
+            const float v = (*s[n])[r], y = v * c1, z = y * y, far = form(v);
+            const float near = y * fmaf(z, fmaf(z, fmaf(z, -17.f / 315.f, 2.f / 15.f), -1.f / 3.f), 1.f);
+            (*s[n])[r] = fabsf(y) <= exact ? near : far;
           }
         rest = Rest{1.f, 0.f, 0.f, 0.f};
       }
@@ -561,6 +563,10 @@ __device__ __forceinline__ void attend_wave(const MaskedArgs& a, const MaskedUni
 // ---------------------------------------------------------------------------
 // few rows: 32 rows a workgroup, its four waves on every fourth tile
 // ---------------------------------------------------------------------------
+//
+// Bound by the bytes of k and v: 16 tokens over 2048 to 8192 keys each, 32 heads over 8 of 128 channels, take 86 us
+// with the merge (4.9 TB/s; a large copy reaches 5.1), one token over 1000 keys 10.5 us, most of it the two launches.
+// A wave keeps two tiles of its own in flight and meets no barrier before the end.
 
 constexpr int kStepWaves = 4;
 constexpr int kStepWindow = 1200;       // bias entries of a wave
@@ -662,8 +668,9 @@ constexpr int kWaveWindow = 1016;       // bias entries of a workgroup, for each
 
 // The order of the workgroups: units (and their parts) in groups of kUnitGroup, in a group the first blocks of all its
 // units first.  Those are the rows that see the most keys (the last ones, which under a causal mask do, or the
-// longest document's), so that the short blocks fill the end of the launch.  Workgroup i runs on XCD i % 8: the blocks of a unit share one L2 where the units of a group are a
-// multiple of 8, and where they are fewer each unit's long and short blocks spread evenly over the XCDs.
+// longest document's), so that the short blocks fill the end of the launch.  Workgroup i runs on XCD i % 8: the blocks
+// of a unit share one L2 where the units of a group are a multiple of 8, and where they are fewer each unit's long and
+// short blocks spread evenly over the XCDs.
 struct BlockOrder {
   int up, at;
   __device__ __forceinline__ BlockOrder(const MaskedArgs& a, int id) {
@@ -848,8 +855,8 @@ struct BlockCore {
   }
 
   // Takes a tile's sum of weights rs; a row whose sum passes the bound (or is inf or NaN) goes over to the tile's
-  // exact max, rescales and weighs again, with the wave's other rows as they were: no row's bits depend on
-  // what rows beside it hold.
+  // exact max, rescales and weighs again, with the wave's other rows as they were, so that no row's reference
+  // point depends on the rows beside it.
   __device__ __forceinline__ void finish(const f32x16& c0, const f32x16& c1, float rs, X8 pb[4]) {
     const bool over = !(rs <= kBound);
     if (__builtin_amdgcn_ballot_w64(over) != 0) {
