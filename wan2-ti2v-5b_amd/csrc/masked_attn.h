@@ -222,9 +222,10 @@ struct TileRange {
 // own, with it tanh(y), y = s scale / cap.  Where all of the wave's |y| are at most 1/4 that is the series
 // y - y^3/3 + 2 y^5/15 - 17 y^7/315, off by 2^-23 at most, in five operations; its usual form 1 - 2 / (1 + e^2y) takes
 // an exponential and a reciprocal, of a quarter of the rate, beside the softmax's own (us a tile of 256 rows, of 128 /
-// 64 channels: 2.35 / 1.77 -> 2.22 / 1.68; uncapped 1.90 / 1.15).  That form is off by 2^-22, which up to caps of 256 is
-// less than the rounding of the softmax weights; beyond, |y| up to 1/4 go by the series beside it too.  (So the scores
-// of the rows beside it may move a capped row's by 2^-22 of the cap; nothing else of a row depends on another.)
+// 64 channels: 2.35 / 1.77 -> 2.25 / 1.70; uncapped 1.90 / 1.20).  That form is off by 2^-22, which up to caps of
+// 256 is less than the rounding of the softmax weights; beyond, |y| up to 1/4 go by the series beside it too.  (So
+// the scores of the rows beside it may move a capped row's by 2^-22 of the cap; nothing else of a row depends on
+// another.)
 // The factor is folded into the exponent; with BIAS value and entry are joined first.
 template <bool CAP, bool BIAS>
 struct ScoreMap {

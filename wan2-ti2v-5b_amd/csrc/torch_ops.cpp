@@ -493,7 +493,8 @@ void linear(const OperatorHandle& op, DispatchKeySet ks, Stack* stack) {
   X("flash_self_attn", flash_self_attn) X("cross_attn", cross_attn) X("self_attn_fused", self_attn_fused) \
   X("self_attn_fused_sumsq", self_attn_fused_sumsq) X("cross_attn_fused", cross_attn_fused)         \
   X("flash_attn_qnorm", flash_attn_qnorm) X("rope", rope_op) X("rms_norm", rms_norm) X("rms_inv", rms_inv) \
-  X("head_norm_rope", head_norm_rope) X("masked_attn", masked_attn) X("adaln", adaln) X("qkv_proj_sumsq", qkv_proj_sumsq) X("linear", linear)
+  X("head_norm_rope", head_norm_rope) X("masked_attn", masked_attn) X("adaln", adaln)               \
+  X("qkv_proj_sumsq", qkv_proj_sumsq) X("linear", linear)
 
 TORCH_LIBRARY_IMPL(wan_hip, CUDA, m) {
 #define WAN_IMPL(name, fn) m.impl(name, torch::CppFunction::makeFromBoxedFunction<&defined<&fn>>());
