@@ -483,9 +483,7 @@ __device__ __forceinline__ void attend_wave(const MaskedArgs& a, const MaskedUni
     kc.issue(t, a.Lk, tiles + slot * (2 * kTile), 0, lane);
     vc.issue(t, a.Lk, tiles + slot * (2 * kTile) + kTile, 0, lane);
   };
-#pragma unroll
-  for (int n = 0; n < SLOTS; ++n)
-    if (t + n * stride < tb) issue(t + n * stride, n);
+  if (t < tb) issue(t, 0);
 
   MaskedOperands<T, HD> op;
   op.init(static_cast<const T*>(a.q.ptr) + u.b * a.q.sb + (int64_t)w.i * a.q.st + (u.h0 + w.g) * a.q.sh, lane);
@@ -503,7 +501,12 @@ __device__ __forceinline__ void attend_wave(const MaskedArgs& a, const MaskedUni
   m_run = -FLT_MAX;
   l_run = 0.f;
 
-  wait_vm_all();      // (as in the block kernel: the query rows are there for the compiler too)
+  // As in the block kernel, the query rows have to be there for the compiler too.  (A wait for all: the second tile goes
+  // out behind it, 256 keys by one workgroup 6.6 -> 6.2 us.)
+  wait_vm_all();
+#pragma unroll
+  for (int n = 1; n < SLOTS; ++n)
+    if (t + n * stride < tb) issue(t + n * stride, n);
   for (int slot = 0; t < tb; t += stride, slot = SLOTS == 1 ? 0 : slot ^ 1) {
     const int kt = t * kWaveKeys;
     const bf16 *Kt = tiles + slot * (2 * kTile), *Vt = Kt + kTile;
@@ -565,9 +568,10 @@ __device__ __forceinline__ void attend_wave(const MaskedArgs& a, const MaskedUni
 // few rows: 32 rows a workgroup, its four waves on every fourth tile
 // ---------------------------------------------------------------------------
 //
-// Bound by the bytes of k and v: 16 tokens over 2048 to 8192 keys each, 32 heads over 8 of 128 channels, take 86 us
-// with the merge (4.9 TB/s; a large copy reaches 5.1), one token over 1000 keys 10.5 us, most of it the two launches.
-// A wave keeps two tiles of its own in flight and meets no barrier before the end.
+// Bound by the bytes of k and v: one token each of 16 samples over 1080 to 8192 keys, 32 heads over 8 of 128
+// channels, takes 85 us with the merge (5.0 TB/s; a large copy reaches 5.1); over 1000 keys of one sample 8.6 us in a
+// replayed graph, most of it the two launches.  A wave keeps two tiles of its own in flight and meets no barrier
+// before the end.
 
 constexpr int kStepWaves = 4;
 constexpr int kStepWindow = 1200;       // bias entries of a wave

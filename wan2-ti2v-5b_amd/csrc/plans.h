@@ -121,11 +121,17 @@ inline MaskedPlan masked_plan(int B, int Hq, int Hk, int Lq, int Lk, int D, bool
     p.by_docs = true;
   };
   if (rows <= kStepRows) {
-    // One workgroup a CU; with key lengths of their own three, if they are left 20 tiles each, so that the long
-    // samples do not end last (us with 1 / 2 / 4 / 6 / 8 parts, 16 samples of 8 k/v heads: 8192 keys 115 / 99 / 110 /
-    // 106 / 112, 2048 to 8192 keys 105 / 78 / 74 / 69 / 71, 1000 keys 20 / 20 / 25 / 30 / 31).
+    // One workgroup a CU, a tile of 32 keys a wave at least (with more than 16 parts two, for the merge), and none
+    // split that reads 128 KB at most (us with 1 / 2 / 4 / 8 / 16 / 32 parts, one token of 32 over 8 heads of 128
+    // channels: 256 keys 6.2 / 7.9 / 7.6 / 7.9 / 8.8, 500 keys 9.4 / 9.9 / 8.2 / 8.5 / 9.3, 1000 keys 14.8 / 12.3 / 9.7 /
+    // 8.6 / 9.4, 4000 keys 45 / 28 / 18 / 12.3 / 10.4 / 10.9; of 8 heads of 64 channels: 500 keys 6.4 / 7.3 / 6.5 / 6.7).
+    // With key lengths of their own three a CU, if they are left 20 tiles each, so that the long samples do not end
+    // last (us with 1 / 2 / 4 / 6 / 8 parts, 16 samples of 8 k/v heads: 8192 keys 115 / 99 / 110 / 106 / 112, 2048 to
+    // 8192 keys 105 / 78 / 74 / 69 / 71, 1000 keys 20 / 20 / 25 / 30 / 31).
     int64_t n = cus / units;
-    if (n > (nt + 3) / 4) n = (nt + 3) / 4;
+    const int fine = (nt + 1) / 2 < 16 ? (nt + 1) / 2 : 16, coarse = (nt + 3) / 4;
+    if (n > (fine > coarse ? fine : coarse)) n = fine > coarse ? fine : coarse;
+    if (nt * D <= 512) n = 1;
     if (ragged && n < 3 * (int64_t)cus / units) {
       const int64_t more = 3 * (int64_t)cus / units < nt / 20 ? 3 * (int64_t)cus / units : nt / 20;
       if (more > n) n = more;
