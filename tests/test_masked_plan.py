@@ -20,6 +20,7 @@ extern "C" void plan(int B, int Hq, int Hk, int Lq, int Lk, int D, int causal, i
                          (long long)p.bytes, p.by_docs};
   for (int i = 0; i < 10; ++i) out[i] = v[i];
 }
+extern "C" int turn(long long workgroups, int cus) { return masked_turn(workgroups, cus); }
 """
 FIELDS = ("pack", "block_rows", "key_groups", "splits", "part_rows", "part_floats", "blocks", "out_rows", "bytes", "by_docs")
 
@@ -36,6 +37,7 @@ def plan(tmp_path_factory):
         out = (ctypes.c_longlong * 10)()
         lib.plan(B, Hq, Hk, Lq, Lk, D, causal, ragged, docs, cus, ctypes.c_size_t(scratch), out)
         return dict(zip(FIELDS, out))
+    call.lib = lib
     return call
 
 
@@ -235,3 +237,18 @@ def test_order_reaches_every_block_once():
             at = inside // size
             seen.add((group * 32 + inside - at * size, at))
         assert seen == {(u, a) for u in range(ups) for a in range(blocks)}
+
+
+@pytest.mark.parametrize("cus", [256, 304, 8, 100])
+def test_turned_workgroups_stay_an_order(plan, cus):
+    turn = plan.lib.turn
+    turn.argtypes = [ctypes.c_longlong, ctypes.c_int]
+    for n in (1, cus - 1, cus, cus + 1, cus + 8, 2 * cus - 1, 2 * cus, 2 * cus + 5, 3 * cus - 1, 3 * cus, 1 << 22):
+        eights = turn(n, cus)
+        assert 0 <= eights <= cus // 8 and cus + 8 * eights <= max(n, cus)
+        ids = []
+        for i in range(min(n, 4 * cus)):
+            turned = (i - cus) >> 3
+            ids.append(cus + (eights - 1 - turned) * 8 + (i & 7) if 0 <= turned < eights else i)
+        assert sorted(ids) == list(range(len(ids)))
+        assert all(a % 8 == b % 8 for a, b in zip(ids, range(len(ids))))      # on the XCD of before

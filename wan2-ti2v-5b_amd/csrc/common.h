@@ -93,7 +93,9 @@ struct FastDiv {
     while ((uint64_t(1) << s) < d) ++s;
     m = (uint32_t)(((uint64_t(1) << (31 + s)) + d - 1) / d);
   }
-  __host__ __device__ __forceinline__ int operator()(int n) const { return (int)((uint64_t(uint32_t(n)) * m) >> (31 + s)); }
+  __host__ __device__ __forceinline__ int operator()(int n) const {
+    return (int)((uint64_t(uint32_t(n)) * m) >> (31 + s));
+  }
 };
 
 struct AnyTensor4 {
@@ -116,8 +118,10 @@ struct MaskedArgs {
   const int32_t* q_start;    // [B] position of query row 0 (null: Lk - Lq)
   float* part;               // scratch of the key split (null: none)
   size_t part_bytes;
-  // set by the launcher (MaskedPlan): blocks of rows of a unit, units of a sample, units times parts, and the divisions by these
+  // set by the launcher (MaskedPlan): blocks of rows of a unit, units of a sample, units times parts, and the divisions
+  // by these
   int pack, splits, part_rows, part_floats, blocks, head_groups, ups;
+  int turn_first, turn_eights;  // 8 turn_eights workgroups from turn_first on are ordered backwards
   bool by_docs;               // blocks begin and end with the large documents
   FastDiv by_pack, by_splits, by_blocks, by_heads, by_group, by_rows, by_last_ups;
 };

@@ -1164,6 +1164,8 @@ int launch_masked_attn(MaskedArgs a, int D, int dtype, hipStream_t s) {
   const int64_t units = (int64_t)a.head_groups * a.B;
   a.blocks = (int)(p.blocks / units);
   a.ups = (int)(units * p.splits);
+  a.turn_first = device_cu_count();
+  a.turn_eights = a.causal && p.slots == 2 ? masked_turn(p.blocks * p.splits, a.turn_first) : 0;
   a.by_pack = FastDiv(a.pack);
   a.by_splits = FastDiv(a.splits);
   a.by_blocks = FastDiv(a.blocks);

@@ -679,6 +679,8 @@ constexpr int kWaveWindow = 1016;       // bias entries of a workgroup, for each
 struct BlockOrder {
   int up, at;
   __device__ __forceinline__ BlockOrder(const MaskedArgs& a, int id) {
+    const int turned = (id - a.turn_first) >> 3;
+    if (turned >= 0 && turned < a.turn_eights) id = a.turn_first + (a.turn_eights - 1 - turned) * 8 + (id & 7);
     const int group = a.by_blocks(id / kUnitGroup), in = id - group * (kUnitGroup * a.blocks);
     // (the last group may be smaller)
     const bool whole = (group + 1) * kUnitGroup <= a.ups;
