@@ -1,7 +1,8 @@
 """MI355X (gfx950) attention hot path of the Wan2.2-TI2V-5B DiT.
 
 Layout of the package:
-  csrc/          HIP kernels (flash attention, QK-RMSNorm / RoPE prep) and the C ABI
+  csrc/          HIP kernels (flash attention, attention under masks, QK-RMSNorm / RoPE prep,
+                 head norms, adaLN, the projection GEMM) and the C ABI
                  declared in include/wan_attn.h, built into libwan_attn.so by build.py
   _native.py     ctypes binding of that C ABI
   ops.py         torch.library custom ops over it (wan_hip::*)

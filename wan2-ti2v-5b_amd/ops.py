@@ -5,6 +5,8 @@ Every op takes bf16 CUDA tensors in the DiT projection layout [B, L, H, 128]
 contiguous), launches on torch's current stream of the tensor's device and
 returns a new contiguous [B, Lq, H, 128] tensor.  Outputs and workspaces come
 from torch's caching allocator; the native side allocates nothing.
+head_norm_rope and masked_attn, which are not of the DiT, take other types,
+head sizes and numbers of k/v heads too.
 
 The fake (meta) kernels let torch.compile trace the ops without running them.
 
