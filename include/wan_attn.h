@@ -123,7 +123,7 @@ int wan_flash_attn_qnorm_ws(wan_tensor q, wan_tensor k, wan_tensor v, wan_tensor
  *   p_i  = q_start[b] + i                  the position of query row i among the keys
  *   s_ij = softmax_scale q_i . k_j;  s = softcap tanh(s / softcap);  s += bias[h, clamp(j - p_i, -R, R) + R]
  *   row i sees key j if j < seqlen_k[b], and j and p_i are of one document, and (causal) j <= p_i or j is
- *   in the first prefix_lens of them
+ *   less than prefix_lens past the document's first position (without documents, past 0)
  *   out_i  = softmax over the keys seen of s_i, times v;  zeros where no key is seen, or all of them at -inf
  * v rows of keys that a row does not see do not reach it, whatever they hold.  The arrays are on the device
  * and int32: values outside their ranges are clamped, doc_starts that do not ascend give other documents,

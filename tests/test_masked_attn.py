@@ -275,6 +275,15 @@ def test_prefix(W, Lq, Lk, Hq, Hk, prefix):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("Lq", [1, 5, 32, 300])
+def test_prefix_of_a_document_that_began_before_the_keys(W, Lq):
+    """The prefix counts from the document's first position, whether or not there is a key."""
+    q, k, v, _ = _make(2, Lq, 300, 4, 2, 64, BF, 17)
+    _check(W, q, k, v, 0.125, causal=True, docs=_ints([[-40, 90, 200], [-7, -2, 30]]),
+           prefix=_ints([[60, 20, 300], [3, 20, 9]]), starts=_ints([0, 300 - Lq]))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype,D", [(BF, 128), (HF, 64)])
 @pytest.mark.parametrize("lens,starts", [([300, 7, 0], None), ([299, 64, 65], [299, 63, 64]), ([-3, 400, 1], [0, 0, 0]),
                                          ([100, 200, 300], [90, 190, 290]), ([300, 300, 300], [-10, 5000, -(2 ** 31)])])

@@ -130,7 +130,7 @@ __device__ __forceinline__ MaskedRow masked_row(const MaskedArgs& a, int b, int 
   r.p = first_position(a, b) + i;
   int len = a.Lk;
   if (a.seqlen_k != nullptr) len = min(max(a.seqlen_k[b], 0), a.Lk);
-  int lo = 0, hi = len, prefix = 0;
+  int lo = 0, hi = len, begin = 0, prefix = 0;      // begin: where the document does, be there a key or not
   bool any = true;
   if (a.doc_starts != nullptr) {
     const int32_t* d = a.doc_starts + (int64_t)b * a.docs;
@@ -147,7 +147,8 @@ __device__ __forceinline__ MaskedRow masked_row(const MaskedArgs& a, int b, int 
     }
     any = n > 0;
     if (any) {
-      lo = max(d[n - 1], 0);
+      begin = d[n - 1];
+      lo = max(begin, 0);
       if (n < a.docs) hi = min(hi, d[n]);
       if (a.prefix_lens != nullptr) prefix = a.prefix_lens[(int64_t)b * a.docs + n - 1];
     }
@@ -155,7 +156,7 @@ __device__ __forceinline__ MaskedRow masked_row(const MaskedArgs& a, int b, int 
     prefix = a.prefix_lens[b];
   }
   if (a.causal) {
-    const int64_t shared = (int64_t)lo + prefix, past = (int64_t)r.p + 1;
+    const int64_t shared = (int64_t)begin + prefix, past = (int64_t)r.p + 1;
     hi = (int)min((int64_t)hi, max(shared, past));
   }
   any = any && lo < hi;

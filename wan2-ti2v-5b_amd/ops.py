@@ -395,8 +395,8 @@ def masked_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, softmax_scale
 
     bias: fp32 [Hq, 2 R + 1].  Row i sees key j if j < seqlen_k[b] (default Lk); if j and p_i are of one
     document, doc_starts [B, n] being the ascending first positions of the documents; and, if causal, if
-    j <= p_i or j is among the first prefix_lens [B] keys (with documents [B, n], of its document).  These are
-    int32.  A row that sees no key is zeros."""
+    j <= p_i or j < prefix_lens [B] (with documents [B, n]: less than that past its document's first position).
+    These are int32.  A row that sees no key is zeros."""
     fn = "masked_attn"
     for name, t in (("q", q), ("k", k), ("v", v)):
         _check_heads(f"{fn}: {name}", t, (64, 128), (torch.bfloat16, torch.float16))
