@@ -978,6 +978,11 @@ __global__ __launch_bounds__(NW * 64, 2) void masked_block_kernel(const MaskedAr
       p_first = at + a.by_pack(row0);
       p_last = at + a.by_pack(rows - 1);
     }
+    auto load_window = [&](int u0) {
+      win.load(a, blk.h0, (range.first + u0) * BK - p_last, (int64_t)(nt - u0 + KG - 1) * BK + (p_last - p_first), window,
+               threadIdx.x, NW * 64);
+    };
+    if constexpr (BIAS) load_window(0);       // (while the tiles are on their way)
     // whether the wave's rows see any key of tile u
     auto seen = [&](int u) {
       const int kt = (range.first + u) * BK;
@@ -995,8 +1000,7 @@ __global__ __launch_bounds__(NW * 64, 2) void masked_block_kernel(const MaskedAr
         const int k0 = (range.first + u0) * BK;
         if (!win.holds(k0 - p_last, k0 + KG * BK - 1 - p_first)) {
           __syncthreads();
-          win.load(a, blk.h0, k0 - p_last, (int64_t)(nt - u0 + KG - 1) * BK + (p_last - p_first), window, threadIdx.x,
-                   NW * 64);
+          load_window(u0);
           __syncthreads();
         }
       }
